@@ -24,7 +24,8 @@ ARCH = os.environ.get("DROID_HIP_ARCH", "gfx950")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 HIP_FLAGS = ["--offload-arch=" + ARCH, "-O3", "-std=c++17", "-fPIC", "-munsafe-fp-atomics",
-             "-Wno-unused-result", "-ffp-contract=fast"]
+             "-Wno-unused-result", "-ffp-contract=fast",
+             "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]      # no packed fp32 instructions (v_pk_*_f32); the host pass does not know the feature and says so
 # DROID_HIP_ABLATION=1: a SECOND, separate build under droid-slam_amd/ablation/ that also carries the prototype kernels
 # (LDS-DMA / Winograd convolutions, first forms of the pyramid build and alt-correlation kernels) and the timing ablations
 # that return wrong results by construction (lookup_mode 2-5, conv_abl).  The shipped library next to this file is built
@@ -60,7 +61,7 @@ if VARIANT:
 SANITIZE = os.environ.get("DROID_HIP_SANITIZE", "0") == "1"
 if SANITIZE:
     assert not ABLATION, "DROID_HIP_SANITIZE and DROID_HIP_ABLATION are separate builds"
-    HIP_FLAGS = [f for f in HIP_FLAGS if f != "-O3"] + ["-O1", "-g", "-fno-omit-frame-pointer", "-fsanitize=address,undefined",
+    HIP_FLAGS = [f for f in HIP_FLAGS if f != "-O3"] + ["-O1", "-g", "-fno-omit-frame-pointer", "-Xarch_host", "-fsanitize=address,undefined",
                                                           "-fno-sanitize-recover=undefined", "-Wno-option-ignored"]
     OUTDIR = os.path.join(HERE, "sanitize")
     OBJ = os.path.join(HERE, "build", "sanitize")
@@ -124,7 +125,7 @@ def build_lib(force=False, verbose=False):
     with ThreadPoolExecutor(max_workers=min(8, max(1, len(jobs)))) as ex:
         list(ex.map(lambda c: _run(c, verbose), jobs))
     if force or jobs or _newer(LIB, objs):
-        _run([HIPCC, "--offload-arch=" + ARCH, "-shared", "-fPIC", "-o", LIB] + (["-fsanitize=address,undefined", "-shared-libsan", "-Wno-option-ignored"] if SANITIZE else []) + objs, verbose)
+        _run([HIPCC, "--offload-arch=" + ARCH, "-shared", "-fPIC", "-o", LIB] + (["-Xarch_host", "-fsanitize=address,undefined", "-shared-libsan", "-Wno-option-ignored"] if SANITIZE else []) + objs, verbose)
     return LIB
 
 
