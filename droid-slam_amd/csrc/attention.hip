@@ -1,0 +1,945 @@
+// Softmax attention over packed sequences of keyframe tokens, forward and backward (gfx950).
+//
+//   o_i = sum_j p_ij v_j,  p_ij = exp(s q_i.k_j - lse_i),  lse_i = log sum_j exp(s q_i.k_j)        over the keys j that row i sees
+//   dV_j = sum_i p_ij dO_i,  dS_ij = p_ij (dO_i.v_j - delta_i),  delta_i = dO_i.o_i,  dQ_i = s sum_j dS_ij k_j,  dK_j = s sum_i dS_ij q_i
+//
+// Rows.  The `group` query heads that share a key head are rows of the same tile: row r = token r / group, head r % group.  Keys and
+// values are then read once for the whole group, a single query of 8 heads still fills a quarter of a 32-row tile, and the gradient of a
+// shared key head is summed inside one workgroup.
+//
+// Products.  v_mfma_f32_32x32x16 with the tile transposed: S^T = K Q^T has one row (query) per lane and 16 keys in its registers, so the
+// softmax statistics are in-lane reductions plus one exchange between the wave's halves, and P^T is already the B operand of
+// O^T = V^T P^T: no trip through LDS.  Register i of lane l holds key 8 (i / 4) + 4 (l / 32) + i % 4 of its 32-key block; a B operand
+// wants 8 consecutive k per lane, which is met by giving A and B the same permutation of the 16 keys of a step (a sum over keys does not
+// care): the transposed reads of V (ds_read_b64_tr_b16: 4 keys x 16 channels per 16 lanes) fetch keys 4 (l / 32) + {0..3, 8..11}.
+//
+// Memory.  64-row tiles arrive by LDS-DMA (buffer_load_dwordx4 ... lds) in two buffers, the next tile under the current one's products;
+// rows behind the end and channels behind head_dim are out of the buffer's range and arrive as zeros.  The 16-byte chunks of a row are
+// stored at chunk ^ swz(row): eight consecutive rows at one chunk (the K operand) and four consecutive rows at two (a transposed read)
+// fall on different banks.
+//
+// Precision.  Products of 16-bit operands accumulate in 32 bits; scores, statistics, p, dP, delta and all accumulators are 32-bit.
+// p and dS are rounded (to nearest) to the inputs' type as operands of the second product: their relative error is the same half step
+// that the rounding of the result has, and averages over the keys.  delta is a difference of large sums where the keys agree: it is formed
+// from o and what its rounding left behind (o_low; one more write and read of o's size), else dQ is off by 1.3 times as much.
+#include "common.h"
+#include <algorithm>
+#include <limits.h>
+#include <math.h>
+#include <string.h>
+#include <type_traits>
+
+namespace {
+using namespace dh;
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) char lds_char;
+
+struct F16 {
+  using V8 = f16x8;
+  // p ~ 1 / (keys) and dS are lifted by 2^4 before they are rounded: 1 / 262144 is still a normal number, and a |dS| of 4094 still finite
+  static constexpr int LIFT = 4;
+  static constexpr unsigned ONE = 0x3c00, INF = 0x7c00;
+  static __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(V8, a), __builtin_bit_cast(V8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ unsigned pack(float x, float y) {
+    f32x2 v; v.x = x; v.y = y;
+    return __builtin_bit_cast(unsigned, __builtin_convertvector(v, f16x2));
+  }
+  static __device__ __forceinline__ float lo(unsigned u) { return (float)__builtin_bit_cast(f16x2, u).x; }
+  static __device__ __forceinline__ float hi(unsigned u) { return (float)__builtin_bit_cast(f16x2, u).y; }
+};
+struct BF16 {
+  using V8 = bf16x8;
+  static constexpr int LIFT = 0;                 // bf16 has the exponent range of fp32
+  static constexpr unsigned ONE = 0x3f80, INF = 0x7f80;
+  static __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(V8, a), __builtin_bit_cast(V8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ unsigned pack(float x, float y) {
+    f32x2 v; v.x = x; v.y = y;
+    return __builtin_bit_cast(unsigned, __builtin_convertvector(v, bf16x2));
+  }
+  static __device__ __forceinline__ float lo(unsigned u) { return __uint_as_float(u << 16); }
+  static __device__ __forceinline__ float hi(unsigned u) { return __uint_as_float(u & 0xffff0000u); }
+};
+
+constexpr int BN = 64;                           // rows of an LDS tile
+constexpr unsigned OUT_OF_RANGE = 0x80000000u;   // byte offset behind every buffer: such lanes of an LDS-DMA write zeros
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr float M_FLOOR = -1e30f;                // start of the running maximum: finite, so that a row without keys makes no inf - inf
+
+struct Item { int q_start, q_len, k_start, k_len, first, begin, end, slot; };   // the plan's record, see dh_attn_plan
+
+struct View { const char* p; long st, sh; };     // base, bytes between tokens, bytes between heads
+
+struct Params {
+  View q, k, v, o, g;                            // o: the forward's output; g: its gradient
+  View dq, dk, dv;
+  char* low;                                     // [q_rows, heads, dim] what the rounding of o left behind, or nothing
+  float* lse;                                    // [q_rows, heads]
+  float* delta;                                  // [q_rows, heads]
+  float* part;                                   // split rows: [slot, kv_heads, rows, DP] and behind them [slot, kv_heads, rows, 2]
+  const Item* items;
+  long n_slots;
+  int kv_heads, group, heads, dim, block, q_rows, k_rows;
+  float c;                                       // scale * log2(e)
+  float scale;
+};
+
+template <int DP> struct Geo {
+  static constexpr int ROWB = DP * 2, CH = DP / 8, TILEB = BN * ROWB;
+  static __device__ __forceinline__ int swz(int r) {
+    const int low = (r >> 3) & 1;
+    if constexpr (DP == 128) return ((r & 7) << 1) | low;
+    else if constexpr (DP == 64) return (((r >> 1) & 3) << 1) | low;
+    else return (((r >> 2) & 1) << 1) | low;
+  }
+};
+
+__device__ __forceinline__ long uniform(long x) {
+  return (long)(((unsigned long)(unsigned)__builtin_amdgcn_readfirstlane((int)((unsigned long)x >> 32)) << 32) |
+                (unsigned)__builtin_amdgcn_readfirstlane((int)x));
+}
+
+// the buffer of everything from `p` on (raw, 2^31 - 1 bytes)
+__device__ __forceinline__ i32x4 buffer_at(const char* p) {
+  const unsigned long a = (unsigned long)p;
+  i32x4 s;
+  s.x = __builtin_amdgcn_readfirstlane((int)a);
+  s.y = __builtin_amdgcn_readfirstlane((int)(a >> 32) & 0xffff);
+  s.z = 0x7fffffff;
+  s.w = 0x00027000;
+  return s;
+}
+
+// lane l copies 16 bytes at buffer + voff (per lane) to LDS address lds + 16 l; zeros where voff is out of range
+__device__ __forceinline__ void dma16(i32x4 buffer, unsigned voff, unsigned lds) {
+  unsigned keep;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds\n\ts_mov_b32 m0, %0"
+               : "=&s"(keep) : "v"(voff), "s"(buffer), "s"(lds) : "memory");
+}
+#define DMA_WAIT_BARRIER() asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory")
+
+// One tensor's 64-row tiles through LDS-DMA by NW waves.  Tile row x is token x / group (from the tile's first token on) and head x % group;
+// a key tensor has group 1.
+template <int DP, int NW> struct TileLoader {
+  using G = Geo<DP>;
+  static constexpr int PER = (BN * G::CH + NW * 64 - 1) / (NW * 64);   // 16-byte chunks a thread
+  static constexpr int STEP = NW * 64 / G::CH;                         // rows between two of them
+  unsigned voff[PER];
+  __device__ __forceinline__ void init(const View& t, int dim, int group, int rows) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int lin = i * NW * 64 + threadIdx.x, r = lin / G::CH, c = (lin % G::CH) ^ G::swz(r), tok = r / group;
+      voff[i] = r < rows && c * 8 < dim ? (unsigned)(tok * t.st + (r - tok * group) * t.sh + c * 16) : OUT_OF_RANGE;
+    }
+  }
+  // `rows`: tile rows that exist
+  __device__ __forceinline__ void issue(const char* tile, int rows, unsigned lds) const {
+    const i32x4 buffer = buffer_at(tile);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = threadIdx.x / G::CH;
+    if (NW * 64 > BN * G::CH && wave * 64 >= BN * G::CH) return;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      dma16(buffer, r + i * STEP < rows ? voff[i] : OUT_OF_RANGE, lds + (i * NW + wave) * 1024);
+  }
+};
+
+// operand rows 32 b .. 32 b + 31 of a tile, channels 16 s + 8 (l / 32) ..: A or B operand of a product over the channels
+template <int DP> __device__ __forceinline__ u32x4 frag(const lds_char* tile, int b, int s, int lane) {
+  using G = Geo<DP>;
+  const int r = lane & 31;
+  return *reinterpret_cast<const __attribute__((address_space(3))) u32x4*>(tile + (b * 32 + r) * G::ROWB + (((2 * s + (lane >> 5)) ^ G::swz(r)) << 4));
+}
+// transposed operand: channel 32 mb + l % 32, tile rows 32 b + 16 ks + 4 (l / 32) + {0..3, 8..11}
+template <int DP> __device__ __forceinline__ u32x4 frag_t(const lds_char* tile, int b, int ks, int mb, int lane) {
+  using G = Geo<DP>;
+  const int x = lane & 15, g = (lane >> 4) & 1, half = lane >> 5;
+  u32x2 part[2];
+#pragma unroll
+  for (int jj = 0; jj < 2; ++jj) {
+    const int r = 8 * jj + 4 * half + (x >> 2);                              // (+ 32 b + 16 ks: no bit that swz looks at)
+    const int c = (2 * (2 * mb + g) + ((x & 3) >> 1)) ^ G::swz(r);
+    typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
+    part[jj] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (lds_i16x4*)(tile + (b * 32 + ks * 16 + r) * G::ROWB + c * 16 + (x & 1) * 8)));
+  }
+  u32x4 v; v.x = part[0].x; v.y = part[0].y; v.z = part[1].x; v.w = part[1].y;
+  return v;
+}
+
+__device__ __forceinline__ float other_half(float v) {                       // the value of lane l ^ 32
+  auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float((threadIdx.x & 32) ? x[0] : x[1]);
+}
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+__device__ __forceinline__ int wave_min(int v) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) v = min(v, __shfl_xor(v, off, 64));
+  return __builtin_amdgcn_readfirstlane(v);
+}
+__device__ __forceinline__ int wave_max(int v) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) v = max(v, __shfl_xor(v, off, 64));
+  return __builtin_amdgcn_readfirstlane(v);
+}
+
+// token i of a sequence sees its first keys_seen keys: all, or up to the end of the block of `block` keys that the token stands in, the last
+// token standing at the last key
+__host__ __device__ __forceinline__ int keys_seen(int i, int q_len, int k_len, int block) {
+  if (block == 0) return k_len;
+  const int at = i + (k_len - q_len);                                        // lengths and block are at most 2^30
+  if (at < 0) return 0;
+  const unsigned e = ((unsigned)at / (unsigned)block + 1) * (unsigned)block;
+  return e < (unsigned)k_len ? (int)e : k_len;
+}
+
+__device__ __forceinline__ bool item_ok(const Item& it, const Params& p) {   // never true of a plan of dh_attn_plan for these tensors
+  return it.q_start >= 0 && it.q_len >= 0 && it.k_start >= 0 && it.k_len >= 0 && it.first >= 0 && it.begin >= 0 &&
+         (long)it.q_start + it.q_len <= p.q_rows && (long)it.k_start + it.k_len <= p.k_rows;
+}
+
+// acc += v^T p over 16 keys of which a row sees those below `lim` (lane's keys: from `key` on 4, and 4 more from key + 8 on).  p is 0 where a
+// key is not seen, and here that also holds for a v that is not finite: such v are left out of the product and added to the rows that see them.
+template <typename T> __device__ __forceinline__ void add_seen(f32x16& acc, u32x4 v, u32x4 p, int key, int lim) {
+  u32x4 kind[3], seen;                           // 1 where v is +inf, -inf, NaN
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int at = key + 2 * (j & 1) + 8 * (j >> 1);
+    seen[j] = (at < lim ? T::ONE : 0u) | (at + 1 < lim ? T::ONE << 16 : 0u);
+    const unsigned x[2] = {v[j] & 0xffffu, v[j] >> 16};
+    unsigned keep = 0u, k0 = 0u, k1 = 0u, k2 = 0u;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const unsigned size = x[h] & 0x7fffu, one = T::ONE << (16 * h);
+      keep |= (size < T::INF ? x[h] : 0u) << (16 * h);
+      k0 |= x[h] == T::INF ? one : 0u;
+      k1 |= x[h] == (T::INF | 0x8000u) ? one : 0u;
+      k2 |= size > T::INF ? one : 0u;
+    }
+    v[j] = keep; kind[0][j] = k0; kind[1][j] = k1; kind[2][j] = k2;
+  }
+  acc = T::mfma(v, p, acc);
+#pragma unroll
+  for (int n = 0; n < 3; ++n) {
+    f32x16 c;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) c[i] = 0.f;
+    c = T::mfma(kind[n], seen, c);
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (c[i] > 0.f) acc[i] += n == 0 ? INFINITY : n == 1 ? -INFINITY : NAN;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------- forward
+// One workgroup: NW x 32 rows (NW * 32 / group tokens) of one key head over the keys [begin, end) of its sequence.  Running maximum and sum
+// per row; the accumulator is only rescaled when a maximum grew by more than 2^8 (p <= 256 until then: exact in 32 bits, and a 16-bit p
+// keeps its relative precision).  slot >= 0: the row range is split over the keys, unnormalised sums go to the workspace for attn_join.
+template <typename T, int DP, int NW>
+__global__ __launch_bounds__(NW * 64, NW == 1 ? 1 : 2) void attn_fwd_kernel(const Params p) {
+  using G = Geo<DP>;
+  __shared__ __attribute__((aligned(1024))) char smem[4 * G::TILEB];         // [buffer][K, V]
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const Item it = p.items[blockIdx.x / p.kv_heads];
+  const int hk = blockIdx.x % p.kv_heads;
+  if (!item_ok(it, p) || it.first >= it.q_len || it.slot >= p.n_slots) return;
+  const int row = wave * 32 + (lane & 31), tpt = NW * 32 / p.group;          // tokens a tile
+  const int tok = it.first + row / p.group, head = hk * p.group + row % p.group;
+  const bool valid = row < tpt * p.group && tok < it.q_len;
+  const int key_end = min(it.end, it.k_len);
+  const int lim = valid ? min(keys_seen(tok, it.q_len, it.k_len, p.block), key_end) : key_end;
+  const int wmin = wave_min(lim), wmax = wave_max(valid ? lim : 0);
+
+  u32x4 qf[DP / 16];
+  {
+    const char* qp = p.q.p + (long)(it.q_start + (valid ? tok : it.first)) * p.q.st + (long)(valid ? head : hk * p.group) * p.q.sh;
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s) {
+      const int d = 16 * s + 8 * (lane >> 5);
+      qf[s] = d < p.dim ? *reinterpret_cast<const u32x4*>(qp + d * 2) : u32x4{0u, 0u, 0u, 0u};
+    }
+  }
+  f32x16 acc[DP / 32];
+  float m, l;                                                                // l: this half's keys only
+  TileLoader<DP, NW> lk, lv;
+  lk.init(p.k, p.dim, 1, BN);
+  lv.init(p.v, p.dim, 1, BN);
+  const char* kp = p.k.p + uniform((long)(it.k_start + it.begin) * p.k.st + (long)hk * p.k.sh);
+  const char* vp = p.v.p + uniform((long)(it.k_start + it.begin) * p.v.st + (long)hk * p.v.sh);
+  lds_char* const lds = (lds_char*)smem;
+  const unsigned lds0 = (unsigned)(unsigned long)lds;
+  const int tiles = (key_end - it.begin + BN - 1) / BN;
+  auto issue = [&](int t) {
+    const unsigned to = lds0 + (t & 1) * 2 * G::TILEB;
+    const int left = key_end - it.begin - t * BN;
+    lk.issue(kp + (long)t * BN * p.k.st, left, to);
+    lv.issue(vp + (long)t * BN * p.v.st, left, to + G::TILEB);
+  };
+  auto walk = [&](auto careful) {
+    constexpr bool CAREFUL = decltype(careful)::value;
+    m = M_FLOOR;
+    l = 0.f;
+#pragma unroll
+    for (int mb = 0; mb < DP / 32; ++mb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[mb][i] = 0.f;
+    if (tiles > 0) issue(0);
+    for (int t = 0; t < tiles; ++t) {
+      DMA_WAIT_BARRIER();                                                      // tile t is there, and everybody has left tile t - 1
+      if (t + 1 < tiles) issue(t + 1);
+      const int n0 = it.begin + t * BN;
+      if (n0 >= wmax) continue;
+      const lds_char* kt = lds + (t & 1) * 2 * G::TILEB;
+      const lds_char* vt = kt + G::TILEB;
+      f32x16 s[2];
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[b][i] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < DP / 16; ++ks)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) s[b] = T::mfma(frag<DP>(kt, b, ks, lane), qf[ks], s[b]);
+      const bool masked = n0 + BN > wmin;
+      if (masked) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (n0 + b * 32 + 8 * (i / 4) + 4 * (lane >> 5) + (i & 3) >= lim) s[b][i] = -INFINITY;
+      }
+      float mx = s[0][0];
+#pragma unroll
+      for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[0][i]);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[1][i]);
+      mx = fmaxf(mx, other_half(mx)) * p.c;
+      if (__any(mx > m + 8.f)) {
+        const float mn = mx > m + 8.f ? mx : m, a = exp2_fast(m - mn);       // (a row's bits do not depend on its neighbours)
+        m = mn;
+        l *= a;
+#pragma unroll
+        for (int mb = 0; mb < DP / 32; ++mb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) acc[mb][i] *= a;
+      }
+      u32x4 pf[2][2];
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          s[b][i] = exp2_fast(fmaf(s[b][i], p.c, -m));
+          l += s[b][i];
+        }
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) pf[b][ks][j] = T::pack(s[b][8 * ks + 2 * j], s[b][8 * ks + 2 * j + 1]);
+      }
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+          for (int mb = 0; mb < DP / 32; ++mb) {
+            const u32x4 vf = frag_t<DP>(vt, b, ks, mb, lane);
+            if (CAREFUL && masked) add_seen<T>(acc[mb], vf, pf[b][ks], n0 + b * 32 + ks * 16 + 4 * (lane >> 5), lim);
+            else acc[mb] = T::mfma(vf, pf[b][ks], acc[mb]);
+          }
+    }
+  };
+  walk(std::false_type());
+  // A value that is not finite makes 0 * v of the rows that do not see it NaN.  Only then the workgroup walks a second time.
+  bool odd = false;
+#pragma unroll
+  for (int mb = 0; mb < DP / 32; ++mb)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) odd |= acc[mb][i] != acc[mb][i];
+  odd = __any(odd && valid);
+  if (NW > 1) {
+    int* flag = reinterpret_cast<int*>(smem);
+    __syncthreads();
+    if (lane == 0) flag[wave] = odd;
+    __syncthreads();
+    odd = false;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) odd |= flag[i] != 0;
+    __syncthreads();
+  }
+  if (odd) walk(std::true_type());
+  l += other_half(l);
+  if (it.slot >= 0) {
+    const long at = (((long)it.slot * p.kv_heads + hk) * (NW * 32) + row);
+    float* po = p.part + at * DP;
+#pragma unroll
+    for (int mb = 0; mb < DP / 32; ++mb)
+#pragma unroll
+      for (int i4 = 0; i4 < 4; ++i4) {
+        f32x4 v; v.x = acc[mb][4 * i4]; v.y = acc[mb][4 * i4 + 1]; v.z = acc[mb][4 * i4 + 2]; v.w = acc[mb][4 * i4 + 3];
+        *reinterpret_cast<f32x4*>(po + mb * 32 + 8 * i4 + 4 * (lane >> 5)) = v;
+      }
+    if (lane < 32) {
+      float* pm = p.part + p.n_slots * p.kv_heads * (NW * 32) * DP + at * 2;
+      pm[0] = m;
+      pm[1] = l;
+    }
+    return;
+  }
+  if (!valid) return;
+  const float inv = l > 0.f || l != l ? 1.f / l : 0.f;                       // nothing seen: zero (NaN stays NaN)
+  char* op = const_cast<char*>(p.o.p) + (long)(it.q_start + tok) * p.o.st + (long)head * p.o.sh;
+  char* lp = p.low + ((long)(it.q_start + tok) * p.heads + head) * p.dim * 2;
+#pragma unroll
+  for (int mb = 0; mb < DP / 32; ++mb)
+#pragma unroll
+    for (int i4 = 0; i4 < 4; ++i4) {
+      const int d = mb * 32 + 8 * i4 + 4 * (lane >> 5);
+      float x[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = acc[mb][4 * i4 + j] * inv;
+      const u32x2 v = {T::pack(x[0], x[1]), T::pack(x[2], x[3])};
+      if (d >= p.dim) continue;
+      *reinterpret_cast<u32x2*>(op + d * 2) = v;
+      if (p.low) *reinterpret_cast<u32x2*>(lp + d * 2) = u32x2{T::pack(x[0] - T::lo(v.x), x[1] - T::hi(v.x)), T::pack(x[2] - T::lo(v.y), x[3] - T::hi(v.y))};
+    }
+  if (lane < 32) p.lse[(long)(it.q_start + tok) * p.heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
+}
+
+// joins the parts of split rows: items {q_start, q_len, -, -, first, first slot, slots, -}; one 32-lane half of a wave per row
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void attn_join_kernel(const Params p, int rows) {
+  const Item it = p.items[blockIdx.y / p.kv_heads];
+  const int hk = blockIdx.y % p.kv_heads;
+  const int row = blockIdx.x * 8 + threadIdx.x / 32, x = threadIdx.x & 31;
+  const int tok = it.first + row / p.group, head = hk * p.group + row % p.group;
+  if (row >= rows / p.group * p.group || tok >= it.q_len || !item_ok(it, p) || (long)it.begin + it.end > p.n_slots) return;
+  const float* pm = p.part + p.n_slots * p.kv_heads * rows * DP;
+  float m = M_FLOOR;
+  for (int i = 0; i < it.end; ++i) m = fmaxf(m, pm[(((long)(it.begin + i) * p.kv_heads + hk) * rows + row) * 2]);
+  float l = 0.f, acc[DP / 32];
+#pragma unroll
+  for (int k = 0; k < DP / 32; ++k) acc[k] = 0.f;
+  for (int i = 0; i < it.end; ++i) {
+    const long at = ((long)(it.begin + i) * p.kv_heads + hk) * rows + row;
+    const float a = exp2f(pm[at * 2] - m);
+    l += a * pm[at * 2 + 1];
+#pragma unroll
+    for (int k = 0; k < DP / 32; ++k) acc[k] += a * p.part[at * DP + k * 32 + x];
+  }
+  const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+  unsigned short* op = reinterpret_cast<unsigned short*>(const_cast<char*>(p.o.p) + (long)(it.q_start + tok) * p.o.st + (long)head * p.o.sh);
+#pragma unroll
+  for (int k = 0; k < DP / 32; ++k)
+    if (k * 32 + x < p.dim) {
+      const unsigned u = T::pack(acc[k] * inv, 0.f);
+      op[k * 32 + x] = (unsigned short)u;
+      if (p.low) reinterpret_cast<unsigned short*>(p.low)[((long)(it.q_start + tok) * p.heads + head) * p.dim + k * 32 + x] = (unsigned short)T::pack(acc[k] * inv - T::lo(u), 0.f);
+    }
+  if (x == 0) p.lse[(long)(it.q_start + tok) * p.heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
+}
+
+// ------------------------------------------------------------------------------------------------------------ backward
+// dQ: the forward's walk over the keys with dO next to Q.  S^T and dP^T = V dO^T give dS^T in the layout of a B operand; the K tile is
+// read a second time transposed for dQ^T = K^T dS^T.  Writes delta for attn_dkv_kernel on the way.
+template <typename T, int DP, int NW>
+__global__ __launch_bounds__(NW * 64, 2) void attn_dq_kernel(const Params p) {
+  using G = Geo<DP>;
+  __shared__ __attribute__((aligned(1024))) char smem[4 * G::TILEB];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const Item it = p.items[blockIdx.x / p.kv_heads];
+  const int hk = blockIdx.x % p.kv_heads;
+  if (!item_ok(it, p) || it.first >= it.q_len || it.slot >= p.n_slots) return;
+  const int row = wave * 32 + (lane & 31), tpt = NW * 32 / p.group;
+  const int tok = it.first + row / p.group, head = hk * p.group + row % p.group;
+  const bool valid = row < tpt * p.group && tok < it.q_len;
+  const int key_end = min(it.end, it.k_len);
+  const int lim = valid ? min(keys_seen(tok, it.q_len, it.k_len, p.block), key_end) : key_end;
+  const int wmin = wave_min(lim), wmax = wave_max(valid ? lim : 0);
+
+  u32x4 qf[DP / 16], gf[DP / 16];
+  const long t_ = it.q_start + (valid ? tok : it.first), h_ = valid ? head : hk * p.group;
+  float delta = 0.f;
+#pragma unroll
+  for (int s = 0; s < DP / 16; ++s) {
+    const int d = 16 * s + 8 * (lane >> 5);
+    const bool in = d < p.dim;
+    qf[s] = in ? *reinterpret_cast<const u32x4*>(p.q.p + t_ * p.q.st + h_ * p.q.sh + d * 2) : u32x4{0u, 0u, 0u, 0u};
+    gf[s] = in ? *reinterpret_cast<const u32x4*>(p.g.p + t_ * p.g.st + h_ * p.g.sh + d * 2) : u32x4{0u, 0u, 0u, 0u};
+    const u32x4 of = in ? *reinterpret_cast<const u32x4*>(p.o.p + t_ * p.o.st + h_ * p.o.sh + d * 2) : u32x4{0u, 0u, 0u, 0u};
+    const u32x4 rf = in && p.low ? *reinterpret_cast<const u32x4*>(p.low + ((t_ * p.heads + h_) * p.dim + d) * 2) : u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) delta += T::lo(gf[s][j]) * (T::lo(of[j]) + T::lo(rf[j])) + T::hi(gf[s][j]) * (T::hi(of[j]) + T::hi(rf[j]));
+  }
+  delta += other_half(delta);
+  const float lse2 = p.lse[t_ * p.heads + h_] * LOG2E - T::LIFT;
+  if (valid && lane < 32) p.delta[t_ * p.heads + h_] = delta;
+
+  f32x16 acc[DP / 32];
+#pragma unroll
+  for (int mb = 0; mb < DP / 32; ++mb)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[mb][i] = 0.f;
+  TileLoader<DP, NW> lk, lv;
+  lk.init(p.k, p.dim, 1, BN);
+  lv.init(p.v, p.dim, 1, BN);
+  const char* kp = p.k.p + uniform((long)(it.k_start + it.begin) * p.k.st + (long)hk * p.k.sh);
+  const char* vp = p.v.p + uniform((long)(it.k_start + it.begin) * p.v.st + (long)hk * p.v.sh);
+  lds_char* const lds = (lds_char*)smem;
+  const unsigned lds0 = (unsigned)(unsigned long)lds;
+  const int tiles = (key_end - it.begin + BN - 1) / BN;
+  auto issue = [&](int t) {
+    const unsigned to = lds0 + (t & 1) * 2 * G::TILEB;
+    const int left = key_end - it.begin - t * BN;
+    lk.issue(kp + (long)t * BN * p.k.st, left, to);
+    lv.issue(vp + (long)t * BN * p.v.st, left, to + G::TILEB);
+  };
+  if (tiles > 0) issue(0);
+  for (int t = 0; t < tiles; ++t) {
+    DMA_WAIT_BARRIER();
+    if (t + 1 < tiles) issue(t + 1);
+    const int n0 = it.begin + t * BN;
+    if (n0 >= wmax) continue;
+    const lds_char* kt = lds + (t & 1) * 2 * G::TILEB;
+    const lds_char* vt = kt + G::TILEB;
+    const bool masked = n0 + BN > wmin;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      f32x16 s, dp;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < DP / 16; ++ks) {
+        s = T::mfma(frag<DP>(kt, b, ks, lane), qf[ks], s);
+        dp = T::mfma(frag<DP>(vt, b, ks, lane), gf[ks], dp);
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] = exp2_fast(fmaf(s[i], p.c, -lse2)) * (dp[i] - delta);
+      if (masked) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (n0 + b * 32 + 8 * (i / 4) + 4 * (lane >> 5) + (i & 3) >= lim) s[i] = 0.f;
+      }
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        u32x4 df;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) df[j] = T::pack(s[8 * ks + 2 * j], s[8 * ks + 2 * j + 1]);
+#pragma unroll
+        for (int mb = 0; mb < DP / 32; ++mb) acc[mb] = T::mfma(frag_t<DP>(kt, b, ks, mb, lane), df, acc[mb]);
+      }
+    }
+  }
+  if (!valid) return;
+  const float f = p.scale * (1.f / (1 << T::LIFT));
+  char* op = const_cast<char*>(p.dq.p) + t_ * p.dq.st + h_ * p.dq.sh;
+#pragma unroll
+  for (int mb = 0; mb < DP / 32; ++mb)
+#pragma unroll
+    for (int i4 = 0; i4 < 4; ++i4) {
+      const int d = mb * 32 + 8 * i4 + 4 * (lane >> 5);
+      u32x2 v;
+      v.x = T::pack(acc[mb][4 * i4] * f, acc[mb][4 * i4 + 1] * f);
+      v.y = T::pack(acc[mb][4 * i4 + 2] * f, acc[mb][4 * i4 + 3] * f);
+      if (d < p.dim) *reinterpret_cast<u32x2*>(op + d * 2) = v;
+    }
+}
+
+// dK, dV: one workgroup holds NW x 32 keys of one key head and walks over the rows (tokens x group) that see them, 64 rows a tile.
+// S = Q K^T and dP = dO V^T have one key per lane, so P and dS are B operands of dV^T = dO^T P and dK^T = Q^T dS.
+template <typename T, int DP, int NW>
+__global__ __launch_bounds__(NW * 64, 2) void attn_dkv_kernel(const Params p) {
+  using G = Geo<DP>;
+  extern __shared__ __attribute__((aligned(1024))) char dyn[];               // [buffer][Q, dO], then [buffer][lse2, delta, end][64]
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const Item it = p.items[blockIdx.x / p.kv_heads];
+  const int hk = blockIdx.x % p.kv_heads;
+  if (!item_ok(it, p) || it.first >= it.k_len) return;
+  const int key = it.first + wave * 32 + (lane & 31);
+  const bool valid = key < it.k_len;
+  u32x4 kf[DP / 16], vf[DP / 16];
+  {
+    const long r = it.k_start + (valid ? key : it.k_len - 1);
+    const char* kp = p.k.p + r * p.k.st + (long)hk * p.k.sh;
+    const char* vp = p.v.p + r * p.v.st + (long)hk * p.v.sh;
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s) {
+      const int d = 16 * s + 8 * (lane >> 5);
+      kf[s] = d < p.dim ? *reinterpret_cast<const u32x4*>(kp + d * 2) : u32x4{0u, 0u, 0u, 0u};
+      vf[s] = d < p.dim ? *reinterpret_cast<const u32x4*>(vp + d * 2) : u32x4{0u, 0u, 0u, 0u};
+    }
+  }
+  f32x16 dk[DP / 32], dv[DP / 32];
+#pragma unroll
+  for (int mb = 0; mb < DP / 32; ++mb)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) dk[mb][i] = dv[mb][i] = 0.f;
+
+  const int tpt = BN / p.group;                                              // tokens a tile
+  TileLoader<DP, NW> lq, lg;
+  lq.init(p.q, p.dim, p.group, tpt * p.group);
+  lg.init(p.g, p.dim, p.group, tpt * p.group);
+  const int tok_end = min(it.end, it.q_len);
+  const int tiles = (tok_end - it.begin + tpt - 1) / tpt;
+  const char* qp = p.q.p + uniform((long)(it.q_start + it.begin) * p.q.st + (long)hk * p.group * p.q.sh);
+  const char* gp = p.g.p + uniform((long)(it.q_start + it.begin) * p.g.st + (long)hk * p.group * p.g.sh);
+  lds_char* const lds = (lds_char*)dyn;
+  const unsigned lds0 = (unsigned)(unsigned long)lds;
+  // row statistics of tile t: 64 threads hold a row each
+  const int mrow = threadIdx.x, mtok = mrow / p.group, mhead = hk * p.group + mrow % p.group;
+  float m_lse = INFINITY, m_delta = 0.f;
+  int m_end = 0;
+  auto fetch = [&](int t) {
+    if (mrow >= BN) return;
+    const int tk = it.begin + t * tpt + mtok;
+    const bool in = mrow < tpt * p.group && tk < tok_end;
+    const long at = (long)(it.q_start + (in ? tk : it.begin)) * p.heads + (in ? mhead : hk * p.group);
+    m_lse = in ? p.lse[at] * LOG2E - T::LIFT : INFINITY;                      // p = 0 in rows that do not exist
+    m_delta = in ? p.delta[at] : 0.f;
+    m_end = in ? keys_seen(tk, it.q_len, it.k_len, p.block) : 0;
+  };
+  auto park = [&](int t) {
+    if (mrow >= BN) return;
+    float* f = reinterpret_cast<float*>(dyn + 4 * G::TILEB) + (t & 1) * 3 * BN + mrow;
+    f[0] = m_lse;
+    f[BN] = m_delta;
+    reinterpret_cast<int*>(f)[2 * BN] = m_end;
+  };
+  auto issue = [&](int t) {
+    const unsigned to = lds0 + (t & 1) * 2 * G::TILEB;
+    const int left = min(tok_end - it.begin - t * tpt, tpt) * p.group;
+    lq.issue(qp + (long)t * tpt * p.q.st, left, to);
+    lg.issue(gp + (long)t * tpt * p.g.st, left, to + G::TILEB);
+  };
+  if (tiles > 0) {
+    fetch(0);
+    issue(0);
+    park(0);
+  }
+  const int wave_key_end = it.first + wave * 32 + 32;
+  for (int t = 0; t < tiles; ++t) {
+    DMA_WAIT_BARRIER();
+    if (t + 1 < tiles) {
+      fetch(t + 1);
+      issue(t + 1);
+    }
+    const lds_char* qt = lds + (t & 1) * 2 * G::TILEB;
+    const lds_char* gt = qt + G::TILEB;
+    const char* stat = dyn + 4 * G::TILEB + (t & 1) * 3 * BN * 4;
+    const int first_tok = it.begin + t * tpt, last_tok = min(first_tok + tpt, tok_end) - 1;
+    // (ends grow with the token) some row of the tile does not see some key of the wave / no row sees any
+    const bool masked = keys_seen(first_tok, it.q_len, it.k_len, p.block) < wave_key_end;
+    if (keys_seen(last_tok, it.q_len, it.k_len, p.block) > it.first + wave * 32) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        f32x16 s, dp;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < DP / 16; ++ks) {
+          s = T::mfma(frag<DP>(qt, b, ks, lane), kf[ks], s);
+          dp = T::mfma(frag<DP>(gt, b, ks, lane), vf[ks], dp);
+        }
+#pragma unroll
+        for (int i4 = 0; i4 < 4; ++i4) {
+          const int r = b * 32 + 8 * i4 + 4 * (lane >> 5);
+          const f32x4 lse2 = *reinterpret_cast<const f32x4*>(stat + r * 4);
+          const f32x4 delta = *reinterpret_cast<const f32x4*>(stat + BN * 4 + r * 4);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int i = 4 * i4 + j;
+            s[i] = exp2_fast(fmaf(s[i], p.c, -lse2[j]));
+            dp[i] = s[i] * (dp[i] - delta[j]);
+          }
+          if (masked) {
+            const i32x4 end = *reinterpret_cast<const i32x4*>(stat + 2 * BN * 4 + r * 4);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (key >= end[j]) s[4 * i4 + j] = dp[4 * i4 + j] = 0.f;
+          }
+        }
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+          u32x4 pf, df;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            pf[j] = T::pack(s[8 * ks + 2 * j], s[8 * ks + 2 * j + 1]);
+            df[j] = T::pack(dp[8 * ks + 2 * j], dp[8 * ks + 2 * j + 1]);
+          }
+#pragma unroll
+          for (int mb = 0; mb < DP / 32; ++mb) {
+            dv[mb] = T::mfma(frag_t<DP>(gt, b, ks, mb, lane), pf, dv[mb]);
+            dk[mb] = T::mfma(frag_t<DP>(qt, b, ks, mb, lane), df, dk[mb]);
+          }
+        }
+      }
+    }
+    if (t + 1 < tiles) park(t + 1);                                          // (its buffer was last read before this iteration's barrier)
+  }
+  if (!valid) return;
+  const float fv = 1.f / (1 << T::LIFT), fk = p.scale * fv;
+  char* kp = const_cast<char*>(p.dk.p) + (long)(it.k_start + key) * p.dk.st + (long)hk * p.dk.sh;
+  char* vp = const_cast<char*>(p.dv.p) + (long)(it.k_start + key) * p.dv.st + (long)hk * p.dv.sh;
+#pragma unroll
+  for (int mb = 0; mb < DP / 32; ++mb)
+#pragma unroll
+    for (int i4 = 0; i4 < 4; ++i4) {
+      const int d = mb * 32 + 8 * i4 + 4 * (lane >> 5);
+      if (d >= p.dim) continue;
+      u32x2 a, b;
+      a.x = T::pack(dk[mb][4 * i4] * fk, dk[mb][4 * i4 + 1] * fk);
+      a.y = T::pack(dk[mb][4 * i4 + 2] * fk, dk[mb][4 * i4 + 3] * fk);
+      b.x = T::pack(dv[mb][4 * i4] * fv, dv[mb][4 * i4 + 1] * fv);
+      b.y = T::pack(dv[mb][4 * i4 + 2] * fv, dv[mb][4 * i4 + 3] * fv);
+      *reinterpret_cast<u32x2*>(kp + d * 2) = a;
+      *reinterpret_cast<u32x2*>(vp + d * 2) = b;
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------- plan
+constexpr int DKV_WAVES = 4;
+constexpr int SLOTS = 512;                       // workgroups the chip holds at two a CU
+constexpr long MAX_ROWS = 1l << 30;
+
+int pad_dim(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
+
+bool heads_ok(int64_t heads, int64_t kv_heads, int64_t dim) {
+  return kv_heads >= 1 && heads >= kv_heads && heads % kv_heads == 0 && heads / kv_heads <= 32 && heads <= 65535 && dim >= 8 && dim <= 128 && dim % 8 == 0;
+}
+
+struct Writer {                                  // counts always, writes where there is room
+  Item* out; long cap, n;
+  void put(const Item& it) { if (out && n < cap) out[n] = it; ++n; }
+};
+
+long cost(const Item& it) { return (long)it.end - it.begin; }
+bool longer(const Item& a, const Item& b) {
+  if (cost(a) != cost(b)) return cost(a) > cost(b);
+  if (a.q_start != b.q_start) return a.q_start < b.q_start;
+  if (a.first != b.first) return a.first < b.first;
+  return a.begin < b.begin;
+}
+
+bool view_ok(const View& t, long tokens, long heads, int dim) {
+  // 16-byte loads; a tile's offsets (64 tokens and the heads of a group) stay below 2^31
+  return t.p && ((unsigned long)t.p & 15) == 0 && t.st >= 0 && t.sh >= 0 && t.st % 16 == 0 && t.sh % 16 == 0 && t.st < (1l << 40) && t.sh < (1l << 40) &&
+         64 * t.st + 32 * t.sh + dim * 2 < (1l << 31);
+}
+
+template <typename T, int DP, int NW> int launch_fwd(const Params& p, long blocks, hipStream_t st) {
+  hipLaunchKernelGGL((attn_fwd_kernel<T, DP, NW>), dim3((unsigned)blocks), dim3(NW * 64), 0, st, p);
+  DH_LAUNCH_CHECK();
+  return DH_OK;
+}
+template <typename T, int DP> int run_fwd(Params p, const dh_attn_info& info, const Item* items, hipStream_t st) {
+  p.items = items;
+  const long blocks = info.n_fwd * info.kv_heads;
+  if (blocks) {
+    const int rc = info.waves == 1 ? launch_fwd<T, DP, 1>(p, blocks, st) : info.waves == 4 ? launch_fwd<T, DP, 4>(p, blocks, st) : launch_fwd<T, DP, 8>(p, blocks, st);
+    if (rc != DH_OK) return rc;
+  }
+  if (info.n_join) {
+    p.items = items + info.n_fwd;
+    const int rows = (int)info.waves * 32;
+    hipLaunchKernelGGL((attn_join_kernel<T, DP>), dim3(rows / 8, (unsigned)(info.n_join * info.kv_heads)), dim3(256), 0, st, p, rows);
+    DH_LAUNCH_CHECK();
+  }
+  return DH_OK;
+}
+template <typename T, int DP> int run_bwd(Params p, const dh_attn_info& info, const Item* items, hipStream_t st) {
+  p.items = items + info.n_fwd + info.n_join;
+  if (info.n_dq) {
+    hipLaunchKernelGGL((attn_dq_kernel<T, DP, 4>), dim3((unsigned)(info.n_dq * info.kv_heads)), dim3(256), 0, st, p);
+    DH_LAUNCH_CHECK();
+  }
+  p.items += info.n_dq;
+  if (info.n_dkv) {
+    const size_t lds = 4 * Geo<DP>::TILEB + 2 * 3 * BN * 4;
+    DH_LDS_OPTIN((attn_dkv_kernel<T, DP, DKV_WAVES>), lds);
+    hipLaunchKernelGGL((attn_dkv_kernel<T, DP, DKV_WAVES>), dim3((unsigned)(info.n_dkv * info.kv_heads)), dim3(DKV_WAVES * 64), lds, st, p);
+    DH_LAUNCH_CHECK();
+  }
+  return DH_OK;
+}
+
+bool info_ok(const dh_attn_info* i) {
+  return i && heads_ok(i->heads, i->kv_heads, i->head_dim) && i->causal_block >= 0 && i->causal_block <= MAX_ROWS && (i->waves == 1 || i->waves == 4 || i->waves == 8) &&
+         i->n_fwd >= 0 && i->n_join >= 0 && i->n_dq >= 0 && i->n_dkv >= 0 && i->n_slots >= 0 && i->q_rows >= 0 && i->k_rows >= 0 && i->q_rows <= MAX_ROWS && i->k_rows <= MAX_ROWS &&
+         i->n_fwd * i->kv_heads <= INT_MAX && i->n_join * i->kv_heads <= 65535 && i->n_dq * i->kv_heads <= INT_MAX && i->n_dkv * i->kv_heads <= INT_MAX;
+}
+
+}  // namespace
+
+extern "C" int dh_attn_plan(const int64_t* q_len, const int64_t* k_len, const int64_t* k_start, int64_t n_seqs, int heads, int kv_heads, int head_dim,
+                            int64_t causal_block, int32_t* plan, int64_t plan_ints, dh_attn_info* info) {
+  if (!info || n_seqs < 0 || (n_seqs && (!q_len || !k_len)) || !heads_ok(heads, kv_heads, head_dim) || causal_block < 0 || plan_ints < 0) return DH_ERR_ARG;
+  const int block = (int)std::min<int64_t>(causal_block, MAX_ROWS), group = heads / kv_heads;
+  long q_rows = 0, k_rows = 0, k_at = 0, most = 0;
+  for (int64_t i = 0; i < n_seqs; ++i) {
+    if (q_len[i] < 0 || k_len[i] < 0 || q_len[i] > MAX_ROWS || k_len[i] > MAX_ROWS) return DH_ERR_ARG;
+    const long ks = k_start ? k_start[i] : k_at;
+    if (ks < 0 || ks > MAX_ROWS) return DH_ERR_ARG;
+    q_rows += q_len[i];
+    k_at += k_len[i];
+    k_rows = std::max(k_rows, ks + (k_len[i] ? k_len[i] : 0));
+    most = std::max<long>(most, q_len[i]);
+    if (q_rows > MAX_ROWS || k_rows > MAX_ROWS || k_at > (1l << 40)) return DH_ERR_ARG;
+  }
+  // rows a workgroup: one wave where a tile of 32 holds every row of the longest sequence (decoding), else 128
+  const int waves = most * group <= 32 ? 1 : 4;
+  const int tpt = waves * 32 / group, tpt_q = 128 / group;
+  long tiles = 0;                                // key tiles of all rows: what there is to spread
+  for (int64_t i = 0; i < n_seqs; ++i)
+    for (long t = 0; t < q_len[i]; t += tpt) {
+      const int e = keys_seen((int)std::min<long>(q_len[i], t + tpt) - 1, (int)q_len[i], (int)k_len[i], block);
+      tiles += (e + BN - 1) / BN * (long)kv_heads;
+    }
+  // few rows over many keys: ranges of keys become work items of their own.  At least 4 tiles each, and only where there is less than one
+  // item for each place on the chip.
+  const long piece = std::max<long>(4, (tiles + SLOTS - 1) / SLOTS);
+  Item* base = reinterpret_cast<Item*>(plan);
+  const long cap = plan ? plan_ints / 8 : 0;
+  Writer w{base, cap, 0};
+  long slots = 0;
+  int64_t counts[4];
+  for (int pass = 0; pass < 4; ++pass) {         // forward items, joins, dQ items, dK / dV items
+    const long from = w.n;
+    long qs = 0, ka = 0, slot = 0;
+    for (int64_t i = 0; i < n_seqs; ++i) {
+      const int m = (int)q_len[i], n = (int)k_len[i];
+      const int ks = (int)(k_start ? k_start[i] : ka);
+      if (pass < 3) {
+        const int step = pass == 2 ? tpt_q : tpt;
+        for (int t = 0; t < m; t += step) {
+          const int e = keys_seen(std::min(m, t + step) - 1, m, n, block);
+          Item it{(int)qs, m, ks, n, t, 0, e, -1};
+          const long nt = (e + BN - 1) / BN;
+          const long pieces = nt > piece + piece / 2 ? (nt + piece - 1) / piece : 1;
+          if (pass == 2 || (pass == 0 && pieces == 1)) w.put(it);
+          else if (pass == 0) {
+            for (long x = 0; x < pieces; ++x) {
+              it.begin = (int)(nt * x / pieces * BN);
+              it.end = (int)std::min<long>(e, nt * (x + 1) / pieces * BN);
+              it.slot = (int)slot++;
+              w.put(it);
+            }
+          } else if (pieces > 1) {
+            it.begin = (int)slot;
+            it.end = (int)pieces;
+            slot += pieces;
+            w.put(it);
+          }
+        }
+      } else {
+        for (int x = 0; x < n; x += DKV_WAVES * 32) {
+          const long t0 = block ? std::max<long>(0, (long)(x / block) * block - (n - m)) : 0;    // the first token that sees key x
+          w.put(Item{(int)qs, m, ks, n, x, (int)std::min<long>(t0, m), m, -1});
+        }
+      }
+      qs += m;
+      ka += n;
+      if (slot > INT_MAX || w.n > INT_MAX / 8) return DH_ERR_ARG;
+    }
+    if (pass == 0) slots = slot;
+    counts[pass] = w.n - from;
+    // longest first, so that the last workgroups to start are short ones
+    if (pass != 1 && base && w.n <= cap) std::sort(base + from, base + w.n, longer);
+  }
+  // key ranges of two sequences that share rows: fine to read, but their gradients would be written twice
+  bool shared = false;
+  if (k_start && n_seqs) {
+    int64_t* order = (int64_t*)malloc(sizeof(int64_t) * n_seqs);
+    if (!order) return DH_ERR_WORKSPACE;
+    int64_t n = 0;
+    for (int64_t i = 0; i < n_seqs; ++i)
+      if (k_len[i]) order[n++] = i;
+    std::sort(order, order + n, [&](int64_t a, int64_t b) { return k_start[a] < k_start[b]; });
+    for (int64_t i = 1; i < n; ++i) shared |= k_start[order[i - 1]] + k_len[order[i - 1]] > k_start[order[i]];
+    free(order);
+  }
+  memset(info, 0, sizeof *info);
+  info->ints = w.n * 8;
+  info->heads = heads; info->kv_heads = kv_heads; info->head_dim = head_dim; info->causal_block = block;
+  info->waves = waves;
+  info->n_fwd = counts[0]; info->n_join = counts[1]; info->n_dq = counts[2]; info->n_dkv = counts[3];
+  info->n_slots = slots; info->q_rows = q_rows; info->k_rows = k_rows; info->keys_shared = shared; info->k_total = k_at;
+  if (!info_ok(info)) return DH_ERR_ARG;
+  if (plan && plan_ints < info->ints) return DH_ERR_WORKSPACE;
+  return DH_OK;
+}
+
+extern "C" size_t dh_attn_fwd_workspace_bytes(const dh_attn_info* info) {
+  if (!info_ok(info)) return 0;
+  return (size_t)info->n_slots * info->kv_heads * (info->waves * 32) * (pad_dim((int)info->head_dim) + 2) * sizeof(float);
+}
+
+extern "C" int dh_attn_fwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh,
+                           void* o, int64_t o_st, int64_t o_sh, void* o_low, float* lse, const int32_t* plan, const dh_attn_info* info, int dtype, int64_t q_rows,
+                           int64_t k_rows, float scale, void* workspace, size_t workspace_bytes, dh_stream_t stream) {
+  if (!info_ok(info) || (dtype != DH_F16 && dtype != DH_BF16) || q_rows < info->q_rows || k_rows < info->k_rows || q_rows > MAX_ROWS || k_rows > MAX_ROWS ||
+      !(scale > 0.f) || !(scale < 1e30f)) return DH_ERR_ARG;
+  if (info->n_fwd == 0) return DH_OK;
+  Params p;
+  memset(&p, 0, sizeof p);
+  p.q = {(const char*)q, q_st * 2, q_sh * 2}; p.k = {(const char*)k, k_st * 2, k_sh * 2}; p.v = {(const char*)v, v_st * 2, v_sh * 2}; p.o = {(const char*)o, o_st * 2, o_sh * 2};
+  const int dim = (int)info->head_dim;
+  if (!plan || !lse || ((unsigned long)o_low & 15) || !view_ok(p.q, q_rows, info->heads, dim) || !view_ok(p.o, q_rows, info->heads, dim)) return DH_ERR_ARG;
+  if (info->k_rows && (!view_ok(p.k, k_rows, info->kv_heads, dim) || !view_ok(p.v, k_rows, info->kv_heads, dim))) return DH_ERR_ARG;
+  if (info->n_slots && (!workspace || ((unsigned long)workspace & 15) || workspace_bytes < dh_attn_fwd_workspace_bytes(info))) return DH_ERR_WORKSPACE;
+  p.low = (char*)o_low; p.lse = lse; p.part = (float*)workspace; p.n_slots = info->n_slots;
+  p.kv_heads = (int)info->kv_heads; p.heads = (int)info->heads; p.group = p.heads / p.kv_heads; p.dim = dim; p.block = (int)info->causal_block;
+  p.q_rows = (int)q_rows; p.k_rows = (int)k_rows; p.scale = scale; p.c = scale * LOG2E;
+  const Item* items = reinterpret_cast<const Item*>(plan);
+  hipStream_t st = (hipStream_t)stream;
+  const int dp = pad_dim(dim);
+  if (dtype == DH_F16) return dp == 32 ? run_fwd<F16, 32>(p, *info, items, st) : dp == 64 ? run_fwd<F16, 64>(p, *info, items, st) : run_fwd<F16, 128>(p, *info, items, st);
+  return dp == 32 ? run_fwd<BF16, 32>(p, *info, items, st) : dp == 64 ? run_fwd<BF16, 64>(p, *info, items, st) : run_fwd<BF16, 128>(p, *info, items, st);
+}
+
+extern "C" size_t dh_attn_bwd_workspace_bytes(const dh_attn_info* info) {
+  return info_ok(info) ? (size_t)info->q_rows * info->heads * sizeof(float) : 0;
+}
+
+extern "C" int dh_attn_bwd(const void* grad, int64_t g_st, int64_t g_sh, const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh,
+                           const void* v, int64_t v_st, int64_t v_sh, const void* o, int64_t o_st, int64_t o_sh, const void* o_low, const float* lse, void* dq, int64_t dq_st,
+                           int64_t dq_sh, void* dk, int64_t dk_st, int64_t dk_sh, void* dv, int64_t dv_st, int64_t dv_sh, const int32_t* plan,
+                           const dh_attn_info* info, int dtype, int64_t q_rows, int64_t k_rows, float scale, void* workspace, size_t workspace_bytes,
+                           dh_stream_t stream) {
+  if (!info_ok(info) || info->keys_shared || (dtype != DH_F16 && dtype != DH_BF16) || q_rows < info->q_rows || k_rows < info->k_rows || q_rows > MAX_ROWS ||
+      k_rows > MAX_ROWS || !(scale > 0.f) || !(scale < 1e30f)) return DH_ERR_ARG;
+  if (info->n_dq == 0 && info->n_dkv == 0) return DH_OK;
+  Params p;
+  memset(&p, 0, sizeof p);
+  p.q = {(const char*)q, q_st * 2, q_sh * 2}; p.k = {(const char*)k, k_st * 2, k_sh * 2}; p.v = {(const char*)v, v_st * 2, v_sh * 2}; p.o = {(const char*)o, o_st * 2, o_sh * 2};
+  p.g = {(const char*)grad, g_st * 2, g_sh * 2}; p.dq = {(const char*)dq, dq_st * 2, dq_sh * 2}; p.dk = {(const char*)dk, dk_st * 2, dk_sh * 2}; p.dv = {(const char*)dv, dv_st * 2, dv_sh * 2};
+  const int dim = (int)info->head_dim;
+  if (!plan) return DH_ERR_ARG;
+  if (info->n_dq) {
+    if (!lse || ((unsigned long)o_low & 15) || !view_ok(p.q, q_rows, info->heads, dim) || !view_ok(p.o, q_rows, info->heads, dim) || !view_ok(p.g, q_rows, info->heads, dim) ||
+        !view_ok(p.dq, q_rows, info->heads, dim)) return DH_ERR_ARG;
+    if (!workspace || workspace_bytes < dh_attn_bwd_workspace_bytes(info)) return DH_ERR_WORKSPACE;
+  }
+  if (info->n_dkv && (!view_ok(p.k, k_rows, info->kv_heads, dim) || !view_ok(p.v, k_rows, info->kv_heads, dim) || !view_ok(p.dk, k_rows, info->kv_heads, dim) ||
+                      !view_ok(p.dv, k_rows, info->kv_heads, dim))) return DH_ERR_ARG;
+  p.low = (char*)const_cast<void*>(o_low); p.lse = const_cast<float*>(lse); p.delta = (float*)workspace;
+  p.kv_heads = (int)info->kv_heads; p.heads = (int)info->heads; p.group = p.heads / p.kv_heads; p.dim = dim; p.block = (int)info->causal_block;
+  p.q_rows = (int)q_rows; p.k_rows = (int)k_rows; p.scale = scale; p.c = scale * LOG2E;
+  const Item* items = reinterpret_cast<const Item*>(plan);
+  hipStream_t st = (hipStream_t)stream;
+  const int dp = pad_dim(dim);
+  if (dtype == DH_F16) return dp == 32 ? run_bwd<F16, 32>(p, *info, items, st) : dp == 64 ? run_bwd<F16, 64>(p, *info, items, st) : run_bwd<F16, 128>(p, *info, items, st);
+  return dp == 32 ? run_bwd<BF16, 32>(p, *info, items, st) : dp == 64 ? run_bwd<BF16, 64>(p, *info, items, st) : run_bwd<BF16, 128>(p, *info, items, st);
+}

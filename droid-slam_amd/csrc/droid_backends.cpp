@@ -9,6 +9,8 @@
 // rejected.
 #include <torch/extension.h>
 #include <c10/hip/HIPStream.h>
+#include <c10/core/DeviceGuard.h>
+#include <ATen/MemoryOverlap.h>
 #include <vector>
 #include <algorithm>
 #include "../../include/droid_hip.h"
@@ -789,6 +791,213 @@ torch::Tensor se3_map(const std::string& op, torch::Tensor a, torch::Tensor X) {
   return Y;
 }
 
+// ---- token operators: packed attention, norm + rotation of query / key heads (include/droid_hip.h dh_attn_*, dh_qk_norm_rope_*) ------
+// These entry points take strided views, run on the tensors' own device (whatever the current one is) and on that device's current stream.
+dh_stream_t stream_of(const torch::Tensor& t) { return (dh_stream_t)c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
+
+int token_dtype(const torch::Tensor& t, const char* name, bool allow_f32) {
+  if (t.scalar_type() == torch::kFloat16) return DH_F16;
+  if (t.scalar_type() == torch::kBFloat16) return DH_BF16;
+  if (allow_f32 && t.scalar_type() == torch::kFloat32) return DH_F32;
+  TORCH_CHECK(false, name, allow_f32 ? " must be float16, bfloat16 or float32" : " must be float16 or bfloat16");
+  return -1;
+}
+void check_heads(const torch::Tensor& t, const char* name, const torch::Tensor& like) {
+  TORCH_CHECK(t.is_cuda(), name, " must be a ROCm device tensor (droid_backends has no CPU path)");
+  TORCH_CHECK(t.dim() == 3, name, " must be [rows, heads, head_dim]");
+  TORCH_CHECK(t.device() == like.device(), name, " is on another device");
+  TORCH_CHECK(t.scalar_type() == like.scalar_type(), name, " has another type");
+}
+int64_t row_stride(const torch::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : 0; }
+int64_t head_stride(const torch::Tensor& t) { return t.size(1) > 1 ? t.stride(1) : 0; }
+#define TOKEN_VIEW(t) t.data_ptr(), row_stride(t), head_stride(t)
+// what dh_attn_* can read in place: adjacent channels, 16-byte pieces, offsets of a tile below 2^31
+bool attn_view(const torch::Tensor& t) {
+  return t.stride(2) == 1 && ((uintptr_t)t.data_ptr() & 15) == 0 && row_stride(t) % 8 == 0 && head_stride(t) % 8 == 0 &&
+         row_stride(t) < (1ll << 24) && 64 * row_stride(t) + 32 * head_stride(t) + t.size(2) < (1ll << 30);
+}
+torch::Tensor attn_input(const torch::Tensor& t) { return t.numel() == 0 || attn_view(t) ? t : t.clone(at::MemoryFormat::Contiguous); }
+
+dh_attn_info attn_info(const torch::Tensor& info) {
+  TORCH_CHECK(info.device().is_cpu() && info.scalar_type() == torch::kInt64 && info.is_contiguous() && info.numel() * 8 == (int64_t)sizeof(dh_attn_info),
+              "info must be what attention_plan returned");
+  dh_attn_info i;
+  memcpy(&i, info.data_ptr<int64_t>(), sizeof i);
+  return i;
+}
+
+// (plan int32 on the host, info int64 on the host)
+std::vector<torch::Tensor> attention_plan(const std::vector<int64_t>& q_len, const std::vector<int64_t>& k_len, c10::optional<std::vector<int64_t>> k_start,
+                                          int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t causal_block) {
+  TORCH_CHECK(q_len.size() == k_len.size() && (!k_start || k_start->size() == q_len.size()), "attention_plan: one key length (and start) for each sequence");
+  TORCH_CHECK(heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && heads / kv_heads <= 32 && heads < 65536, "attention_plan: heads must be a multiple (up to 32) of kv_heads");
+  TORCH_CHECK(head_dim >= 8 && head_dim <= 128 && head_dim % 8 == 0, "attention_plan: head_dim must be a multiple of 8 up to 128");
+  TORCH_CHECK(causal_block >= 0, "attention_plan: causal_block must not be negative");
+  dh_attn_info i;
+  const int64_t* ks = k_start ? k_start->data() : nullptr;
+  check_status(dh_attn_plan(q_len.data(), k_len.data(), ks, (int64_t)q_len.size(), (int)heads, (int)kv_heads, (int)head_dim, causal_block, nullptr, 0, &i),
+               "attention_plan (lengths and starts must not be negative, rows at most 2^30)");
+  torch::Tensor plan = torch::empty({i.ints}, torch::kInt32), info = torch::empty({(int64_t)(sizeof i / 8)}, torch::kInt64);
+  check_status(dh_attn_plan(q_len.data(), k_len.data(), ks, (int64_t)q_len.size(), (int)heads, (int)kv_heads, (int)head_dim, causal_block,
+                            plan.data_ptr<int32_t>(), i.ints, &i), "attention_plan");
+  memcpy(info.data_ptr<int64_t>(), &i, sizeof i);
+  return {plan, info};
+}
+
+void check_attn(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& plan, const dh_attn_info& i, const char* what) {
+  check_heads(q, "q", q); check_heads(k, "k", q); check_heads(v, "v", q);
+  TORCH_CHECK(q.size(1) == i.heads && k.size(1) == i.kv_heads && q.size(2) == i.head_dim && k.size(2) == i.head_dim && v.sizes() == k.sizes(), what,
+              ": q must be [rows, ", i.heads, ", ", i.head_dim, "], k and v [rows, ", i.kv_heads, ", ", i.head_dim, "] as the plan says");
+  TORCH_CHECK(q.size(0) >= i.q_rows, what, ": the plan has ", i.q_rows, " query rows, q has ", q.size(0));
+  TORCH_CHECK(k.size(0) >= i.k_rows, what, ": the plan has ", i.k_rows, " key rows, k has ", k.size(0));
+  TORCH_CHECK(plan.device() == q.device() && plan.scalar_type() == torch::kInt32 && plan.is_contiguous() && plan.numel() == i.ints, what, ": the plan is on another device");
+}
+
+// {o [rows, heads, head_dim], lse [rows, heads] f32, o_low (for_backward: what the rounding of o left behind; else empty)}; rows behind the last sequence are 0 / -inf, or left alone in an `out` of the caller's
+std::vector<torch::Tensor> attention_forward(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor plan, torch::Tensor info, double scale,
+                                             c10::optional<torch::Tensor> out, bool for_backward) {
+  const dh_attn_info i = attn_info(info);
+  check_attn(q, k, v, plan, i, "attention_forward");
+  const int dt = token_dtype(q, "q", false);
+  TORCH_CHECK(scale > 0 && scale < 1e30, "attention_forward: scale must be positive");
+  const c10::DeviceGuard guard(q.device());
+  torch::Tensor o = out ? *out : torch::empty(q.sizes(), q.options());
+  torch::Tensor lse = torch::empty({q.size(0), q.size(1)}, q.options().dtype(torch::kFloat32));
+  torch::Tensor low = for_backward ? torch::empty(q.sizes(), q.options()) : torch::empty({0}, q.options());
+  if (out) {
+    check_heads(o, "out", q);
+    TORCH_CHECK(o.sizes() == q.sizes() && attn_view(o), "out must have q's shape, adjacent channels and 16-byte aligned heads");
+    at::assert_no_internal_overlap(o);
+    at::assert_no_overlap(o, q); at::assert_no_overlap(o, k); at::assert_no_overlap(o, v);
+  }
+  q = attn_input(q); k = attn_input(k); v = attn_input(v);
+  const size_t wsb = dh_attn_fwd_workspace_bytes(&i);
+  torch::Tensor ws = torch::empty({(int64_t)wsb}, q.options().dtype(torch::kUInt8));
+  check_status(dh_attn_fwd(TOKEN_VIEW(q), TOKEN_VIEW(k), TOKEN_VIEW(v), TOKEN_VIEW(o), for_backward ? low.data_ptr() : nullptr, lse.data_ptr<float>(),
+                           plan.data_ptr<int32_t>(), &i, dt, q.size(0), k.size(0), (float)scale, ws.data_ptr(), wsb, stream_of(q)), "attention_forward");
+  if (q.size(0) > i.q_rows) {
+    if (!out) o.narrow(0, i.q_rows, q.size(0) - i.q_rows).zero_();
+    lse.narrow(0, i.q_rows, q.size(0) - i.q_rows).fill_(-std::numeric_limits<float>::infinity());
+  }
+  return {o, lse, low};
+}
+
+// {dq, dk, dv}, zero in rows that belong to no sequence
+std::vector<torch::Tensor> attention_backward(torch::Tensor grad, torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor o, torch::Tensor lse,
+                                              c10::optional<torch::Tensor> low, torch::Tensor plan, torch::Tensor info, double scale) {
+  const dh_attn_info i = attn_info(info);
+  check_attn(q, k, v, plan, i, "attention_backward");
+  check_heads(o, "o", q); check_heads(grad, "grad", q);
+  TORCH_CHECK(o.sizes() == q.sizes() && grad.sizes() == q.sizes(), "attention_backward: o and grad must have q's shape");
+  TORCH_CHECK(lse.device() == q.device() && lse.scalar_type() == torch::kFloat32 && lse.is_contiguous() && lse.dim() == 2 && lse.size(0) == q.size(0) && lse.size(1) == q.size(1),
+              "attention_backward: lse must be what attention_forward returned");
+  if (low) check_heads(*low, "o_low", q);
+  TORCH_CHECK(!low || (low->sizes() == q.sizes() && low->is_contiguous()), "attention_backward: o_low must be what attention_forward returned");
+  TORCH_CHECK(!i.keys_shared, "attention_backward: two sequences of the plan share keys");
+  const int dt = token_dtype(q, "q", false);
+  TORCH_CHECK(scale > 0 && scale < 1e30, "attention_backward: scale must be positive");
+  const c10::DeviceGuard guard(q.device());
+  q = attn_input(q); k = attn_input(k); v = attn_input(v); o = attn_input(o); grad = attn_input(grad);
+  const bool gaps = i.k_total < i.k_rows;
+  torch::Tensor dq = torch::empty(q.sizes(), q.options());
+  torch::Tensor dk = gaps ? torch::zeros(k.sizes(), k.options()) : torch::empty(k.sizes(), k.options());
+  torch::Tensor dv = gaps ? torch::zeros(k.sizes(), k.options()) : torch::empty(k.sizes(), k.options());
+  const size_t wsb = dh_attn_bwd_workspace_bytes(&i);
+  torch::Tensor ws = torch::empty({(int64_t)wsb}, q.options().dtype(torch::kUInt8));
+  check_status(dh_attn_bwd(TOKEN_VIEW(grad), TOKEN_VIEW(q), TOKEN_VIEW(k), TOKEN_VIEW(v), TOKEN_VIEW(o), low ? low->data_ptr() : nullptr, lse.data_ptr<float>(), TOKEN_VIEW(dq), TOKEN_VIEW(dk), TOKEN_VIEW(dv),
+                           plan.data_ptr<int32_t>(), &i, dt, q.size(0), k.size(0), (float)scale, ws.data_ptr(), wsb, stream_of(q)), "attention_backward");
+  if (q.size(0) > i.q_rows) dq.narrow(0, i.q_rows, q.size(0) - i.q_rows).zero_();
+  if (!gaps && k.size(0) > i.k_rows) {
+    dk.narrow(0, i.k_rows, k.size(0) - i.k_rows).zero_();
+    dv.narrow(0, i.k_rows, k.size(0) - i.k_rows).zero_();
+  }
+  return {dq, dk, dv};
+}
+
+struct RopeArgs { std::vector<int> sections; int pos_type, w_dtype; const void *qw, *kw; };
+RopeArgs rope_args(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& positions, const torch::Tensor& inv_freq, const std::vector<int64_t>& sections,
+                   const c10::optional<torch::Tensor>& q_weight, const c10::optional<torch::Tensor>& k_weight, bool normalize, double eps) {
+  check_heads(q, "q", q); check_heads(k, "k", q);
+  TORCH_CHECK(k.size(0) == q.size(0) && k.size(2) == q.size(2), "q and k must have the same tokens and head_dim");
+  const int64_t d = q.size(2);
+  TORCH_CHECK(d >= 2 && d <= 256 && d % 2 == 0, "head_dim must be even and at most 256");
+  TORCH_CHECK(!sections.empty() && sections.size() <= 4, "one to four sections");
+  RopeArgs a{{}, 0, DH_F32, nullptr, nullptr};
+  int64_t pairs = 0;
+  for (const int64_t s : sections) {
+    TORCH_CHECK(s >= 0 && s <= d, "sections must not be negative");
+    a.sections.push_back((int)s);
+    pairs += s;
+  }
+  TORCH_CHECK(pairs <= d / 2, "the sections have ", pairs, " pairs, a head has ", d / 2);
+  TORCH_CHECK(positions.device() == q.device() && positions.is_contiguous() && positions.numel() == q.size(0) * (int64_t)sections.size() && positions.dim() <= 2 &&
+              positions.dim() >= 1 && positions.size(0) == q.size(0), "positions must be contiguous [tokens, axes] on q's device");
+  a.pos_type = positions.scalar_type() == torch::kInt32 ? 0 : positions.scalar_type() == torch::kInt64 ? 1 : positions.scalar_type() == torch::kFloat32 ? 2 : -1;
+  TORCH_CHECK(a.pos_type >= 0, "positions must be int32, int64 or float32");
+  TORCH_CHECK(inv_freq.device() == q.device() && inv_freq.scalar_type() == torch::kFloat32 && inv_freq.is_contiguous() && inv_freq.numel() == pairs,
+              "inv_freq must be contiguous float32 with one value for each pair of the sections, on q's device");
+  TORCH_CHECK(normalize || (!q_weight && !k_weight), "weights need normalize");
+  TORCH_CHECK(eps >= 0, "eps must not be negative");
+  const torch::Tensor* first = nullptr;
+  for (const auto* w : {&q_weight, &k_weight})
+    if (*w) {
+      const torch::Tensor& t = **w;
+      TORCH_CHECK(t.device() == q.device() && t.dim() == 1 && t.size(0) == d && t.is_contiguous(), "weights must be contiguous [head_dim] on q's device");
+      TORCH_CHECK(!first || first->scalar_type() == t.scalar_type(), "q_weight and k_weight must have one type");
+      a.w_dtype = token_dtype(t, "weights", true);
+      first = &t;
+      (w == &q_weight ? a.qw : a.kw) = t.data_ptr();
+    }
+  return a;
+}
+torch::Tensor rope_input(const torch::Tensor& t) { return t.numel() == 0 || t.stride(2) == 1 ? t : t.contiguous(); }
+
+void rope_status(int rc, const char* what) {
+  TORCH_CHECK(rc != DH_ERR_UNSUPPORTED, what, ": a head of more than 128 channels needs even halves (pairs, resting channels, strides)");
+  check_status(rc, what);
+}
+
+std::vector<torch::Tensor> qk_norm_rope_forward(torch::Tensor q, torch::Tensor k, torch::Tensor positions, torch::Tensor inv_freq, const std::vector<int64_t>& sections,
+                                                c10::optional<torch::Tensor> q_weight, c10::optional<torch::Tensor> k_weight, bool normalize, double eps, bool interleaved,
+                                                c10::optional<torch::Tensor> q_out, c10::optional<torch::Tensor> k_out) {
+  const RopeArgs a = rope_args(q, k, positions, inv_freq, sections, q_weight, k_weight, normalize, eps);
+  const int dt = token_dtype(q, "q", true);
+  const c10::DeviceGuard guard(q.device());
+  torch::Tensor qo = q_out ? *q_out : torch::empty(q.sizes(), q.options()), ko = k_out ? *k_out : torch::empty(k.sizes(), k.options());
+  check_heads(qo, "q_out", q); check_heads(ko, "k_out", q);
+  TORCH_CHECK(qo.sizes() == q.sizes() && ko.sizes() == k.sizes() && (qo.numel() == 0 || qo.stride(2) == 1) && (ko.numel() == 0 || ko.stride(2) == 1),
+              "q_out / k_out must have the shapes of q / k and adjacent channels");
+  at::assert_no_internal_overlap(qo); at::assert_no_internal_overlap(ko);
+  at::assert_no_partial_overlap(qo, q); at::assert_no_partial_overlap(ko, k);
+  at::assert_no_overlap(qo, k); at::assert_no_overlap(ko, q); at::assert_no_overlap(qo, ko);
+  q = rope_input(q); k = rope_input(k);
+  rope_status(dh_qk_norm_rope_fwd(TOKEN_VIEW(q), TOKEN_VIEW(k), TOKEN_VIEW(qo), TOKEN_VIEW(ko), positions.data_ptr(), a.pos_type,
+                                  inv_freq.data_ptr<float>(), a.sections.data(), (int)a.sections.size(), a.qw, a.kw, a.w_dtype, dt, q.size(0), (int)q.size(1), (int)k.size(1),
+                                  (int)q.size(2), normalize, (float)eps, interleaved, stream_of(q)), "qk_norm_rope_forward");
+  return {qo, ko};
+}
+
+// {dq, dk, dq_weight, dk_weight}; the weights' gradients are empty where there is no weight
+std::vector<torch::Tensor> qk_norm_rope_backward(torch::Tensor dq_out, torch::Tensor dk_out, torch::Tensor q, torch::Tensor k, torch::Tensor positions, torch::Tensor inv_freq,
+                                                 const std::vector<int64_t>& sections, c10::optional<torch::Tensor> q_weight, c10::optional<torch::Tensor> k_weight,
+                                                 bool normalize, double eps, bool interleaved) {
+  const RopeArgs a = rope_args(q, k, positions, inv_freq, sections, q_weight, k_weight, normalize, eps);
+  check_heads(dq_out, "dq_out", q); check_heads(dk_out, "dk_out", q);
+  TORCH_CHECK(dq_out.sizes() == q.sizes() && dk_out.sizes() == k.sizes(), "the gradients must have the shapes of q and k");
+  const int dt = token_dtype(q, "q", true);
+  const c10::DeviceGuard guard(q.device());
+  q = rope_input(q); k = rope_input(k); dq_out = rope_input(dq_out); dk_out = rope_input(dk_out);
+  torch::Tensor dq = torch::empty(q.sizes(), q.options()), dk = torch::empty(k.sizes(), k.options());
+  torch::Tensor dqw = q_weight ? torch::empty_like(*q_weight) : torch::empty({0}, q.options()), dkw = k_weight ? torch::empty_like(*k_weight) : torch::empty({0}, q.options());
+  const size_t wsb = q_weight || k_weight ? dh_qk_norm_rope_bwd_workspace_bytes((int)q.size(2)) : 0;
+  torch::Tensor ws = torch::empty({(int64_t)wsb}, q.options().dtype(torch::kUInt8));
+  rope_status(dh_qk_norm_rope_bwd(TOKEN_VIEW(dq_out), TOKEN_VIEW(dk_out), TOKEN_VIEW(q), TOKEN_VIEW(k), TOKEN_VIEW(dq), TOKEN_VIEW(dk), q_weight ? dqw.data_ptr() : nullptr,
+                                  k_weight ? dkw.data_ptr() : nullptr, positions.data_ptr(), a.pos_type, inv_freq.data_ptr<float>(), a.sections.data(), (int)a.sections.size(),
+                                  a.qw, a.kw, a.w_dtype, dt, q.size(0), (int)q.size(1), (int)k.size(1), (int)q.size(2), normalize, (float)eps, interleaved, ws.data_ptr(), wsb,
+                                  stream_of(q)), "qk_norm_rope_backward");
+  return {dq, dk, dqw, dkw};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -857,6 +1066,17 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("reproject", &reproject, "fused reprojection (Python thresholds)");
   m.def("se3_op", &se3_op, "SE3 inv/mul/exp/retr");
   m.def("se3_map", &se3_map, "SE3 act4/adjT");
+  m.def("attention_plan", &attention_plan, "work items of packed attention for one set of lengths", py::arg("q_lengths"), py::arg("k_lengths"), py::arg("k_starts"),
+        py::arg("heads"), py::arg("kv_heads"), py::arg("head_dim"), py::arg("causal_block") = 0);
+  m.def("attention_forward", &attention_forward, "packed softmax attention: {o, lse, o_low}", py::arg("q"), py::arg("k"), py::arg("v"), py::arg("plan"), py::arg("info"),
+        py::arg("scale"), py::arg("out") = py::none(), py::arg("for_backward") = false);
+  m.def("attention_backward", &attention_backward, "gradients of packed softmax attention: {dq, dk, dv}");
+  m.def("qk_norm_rope_forward", &qk_norm_rope_forward, "norm of query / key heads and rotation by position: {q, k}", py::arg("q"), py::arg("k"), py::arg("positions"),
+        py::arg("inv_freq"), py::arg("sections"), py::arg("q_weight") = py::none(), py::arg("k_weight") = py::none(), py::arg("normalize") = true, py::arg("eps") = 1e-6,
+        py::arg("interleaved") = false, py::arg("q_out") = py::none(), py::arg("k_out") = py::none());
+  m.def("qk_norm_rope_backward", &qk_norm_rope_backward, "gradients of qk_norm_rope_forward: {dq, dk, dq_weight, dk_weight}", py::arg("dq_out"), py::arg("dk_out"),
+        py::arg("q"), py::arg("k"), py::arg("positions"), py::arg("inv_freq"), py::arg("sections"), py::arg("q_weight") = py::none(), py::arg("k_weight") = py::none(),
+        py::arg("normalize") = true, py::arg("eps") = 1e-6, py::arg("interleaved") = false);
   m.def("version", []() { return std::string(dh_version()); });
   m.def("set_option", [](const std::string& name, int value) { check_status(dh_set_option(name.c_str(), value), "set_option"); });
   m.def("options_epoch", []() { return dh_options_epoch(); });

@@ -37,6 +37,7 @@ extern "C" {
 /* element types of correlation volumes / feature maps */
 #define DH_F16 0
 #define DH_F32 1
+#define DH_BF16 3  /* dh_attn_* and dh_qk_norm_rope_* only */
 #define DH_F64 2   /* dh_corr_index_fwd / _bwd only (the reference dispatches double there too, correlation_kernels.cu:146,167) */
 
 typedef void* dh_stream_t;
@@ -469,6 +470,73 @@ int dh_reproject(const float* poses, const float* disps, const float* intrinsics
 int dh_reproject_ex(const float* poses, const float* disps, const float* intrinsics, int per_frame_intrinsics,
                     const int64_t* ii, const int64_t* jj, float* coords, float* valid,
                     int E, int ht, int wd, dh_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * Softmax attention over packed sequences of tokens (keyframe feature maps, frame by frame, row by row), forward and backward.
+ *   q, o, grad, dq [q_rows, heads, head_dim], k, v, dk, dv [k_rows, kv_heads, head_dim], DH_F16 or DH_BF16; *_st / *_sh = elements between
+ *   tokens / heads (channels adjacent; bases 16-byte aligned, strides multiples of 8 and >= 0, 64 * st + 32 * sh below 2^30 elements).
+ *   heads % kv_heads == 0 and heads / kv_heads <= 32: query head h reads key head h / (heads / kv_heads).  head_dim a multiple of 8 up to 128.
+ * Sequence n has q_len[n] consecutive rows of q (packed one behind the other from row 0 on) and k_len[n] consecutive rows of k / v from row
+ * k_start[n] on (k_start NULL: packed as well).  Its token i sees its first e(i) keys: all k_len (causal_block 0), or
+ * min(k_len, (floor((i + k_len - q_len) / causal_block) + 1) * causal_block): 1 = token by token, the last token standing at the last key;
+ * n = whole blocks (keyframes) of n keys.  A row that sees nothing: o = 0, lse = -inf, gradients 0.
+ *   o = softmax(scale q k^T) v (scale > 0), lse [q_rows, heads] f32 = natural logarithm of the row's sum.
+ * Rows of o, lse, dq behind the last sequence, and rows of dk, dv that belong to no sequence, are left as they were.
+ * Values are expected to be finite where a gradient is wanted.  A non-finite value (q, k or v) reaches the rows that see it and no others.
+ *
+ * dh_attn_plan runs on the HOST: it lays out the work items of one set of lengths.  plan_host NULL: only fills *info (info->ints = ints
+ * wanted); else writes plan_host[0 .. info->ints).  The caller copies it to the device and passes it, with *info, to every call on these
+ * lengths.  Rows split over their keys (few rows, long key ranges) meet in the workspace.
+ * o_low [q_rows, heads, head_dim] dense, or NULL: what the rounding of o to 16 bits left behind; the backward's row sums are formed from both.
+ * dh_attn_bwd takes o, o_low and lse of the forward call with the same scale; sequences must not share keys (DH_ERR_ARG).  It is deterministic:
+ * no atomics; two calls on the same values give the same bits.
+ */
+typedef struct {
+  int64_t ints;                                         /* length of the plan */
+  int64_t heads, kv_heads, head_dim, causal_block;
+  int64_t waves;                                        /* wavefronts (32 rows each) of a forward workgroup */
+  int64_t n_fwd, n_join, n_dq, n_dkv, n_slots;          /* work items; partial results of split rows */
+  int64_t q_rows, k_rows;                               /* rows that q and k must have at least */
+  int64_t k_total;                                      /* sum of k_len */
+  int64_t keys_shared;                                  /* two sequences share keys: no backward */
+} dh_attn_info;
+int dh_attn_plan(const int64_t* q_len_host, const int64_t* k_len_host, const int64_t* k_start_host, int64_t n_seqs,
+                 int heads, int kv_heads, int head_dim, int64_t causal_block, int32_t* plan_host, int64_t plan_ints, dh_attn_info* info_host);
+size_t dh_attn_fwd_workspace_bytes(const dh_attn_info* info_host);
+size_t dh_attn_bwd_workspace_bytes(const dh_attn_info* info_host);
+int dh_attn_fwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh,
+                const void* v, int64_t v_st, int64_t v_sh, void* o, int64_t o_st, int64_t o_sh, void* o_low, float* lse,
+                const int32_t* plan, const dh_attn_info* info_host, int dtype, int64_t q_rows, int64_t k_rows, float scale,
+                void* workspace, size_t workspace_bytes, dh_stream_t stream);
+int dh_attn_bwd(const void* grad, int64_t g_st, int64_t g_sh, const void* q, int64_t q_st, int64_t q_sh,
+                const void* k, int64_t k_st, int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh,
+                const void* o, int64_t o_st, int64_t o_sh, const void* o_low, const float* lse,
+                void* dq, int64_t dq_st, int64_t dq_sh, void* dk, int64_t dk_st, int64_t dk_sh, void* dv, int64_t dv_st, int64_t dv_sh,
+                const int32_t* plan, const dh_attn_info* info_host, int dtype, int64_t q_rows, int64_t k_rows, float scale,
+                void* workspace, size_t workspace_bytes, dh_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * Norm of every query and key head and rotation by the token's position, in one pass, forward and backward.
+ *   q, q_out, dq_out, dq [tokens, heads, head_dim], k ... [tokens, kv_heads, head_dim], DH_F16, DH_BF16 or DH_F32; *_st / *_sh = elements
+ *   between tokens / heads, >= 0 (channels adjacent).  q_out may be q itself, k_out k itself (the same elements, not shifted ones).
+ *   positions [tokens, n_axes]: pos_type 0 = int32, 1 = int64, 2 = float; inv_freq [sum of sections] f32; 1 <= n_axes <= 4.
+ * z = x / sqrt(mean(x^2) + eps) * weight (normalize; weight [head_dim] of w_dtype, NULL = ones) or z = x (no weights then).  The first
+ * sections[0] pairs turn by positions[:,0] * inv_freq[pair], the next sections[1] by positions[:,1], ...: (a, b) -> (a cos - b sin,
+ * a sin + b cos); with P = sum of sections a pair is (i, P + i), or (2i, 2i + 1) where `interleaved`; channels from 2 P on do not turn.
+ * Angles are exact to 32 bits at any position.  head_dim even, up to 256 (above 128 the halves must be even: DH_ERR_UNSUPPORTED).
+ * Backward: x is only read where `normalize`; dq_weight / dk_weight [head_dim] of w_dtype or NULL; no atomics. */
+int dh_qk_norm_rope_fwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh,
+                        void* q_out, int64_t qo_st, int64_t qo_sh, void* k_out, int64_t ko_st, int64_t ko_sh,
+                        const void* positions, int pos_type, const float* inv_freq, const int* sections_host, int n_axes,
+                        const void* q_weight, const void* k_weight, int w_dtype, int dtype, int64_t tokens, int heads, int kv_heads,
+                        int head_dim, int normalize, float eps, int interleaved, dh_stream_t stream);
+size_t dh_qk_norm_rope_bwd_workspace_bytes(int head_dim);
+int dh_qk_norm_rope_bwd(const void* dq_out, int64_t gq_st, int64_t gq_sh, const void* dk_out, int64_t gk_st, int64_t gk_sh,
+                        const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh,
+                        void* dq, int64_t dq_st, int64_t dq_sh, void* dk, int64_t dk_st, int64_t dk_sh, void* dq_weight, void* dk_weight,
+                        const void* positions, int pos_type, const float* inv_freq, const int* sections_host, int n_axes,
+                        const void* q_weight, const void* k_weight, int w_dtype, int dtype, int64_t tokens, int heads, int kv_heads,
+                        int head_dim, int normalize, float eps, int interleaved, void* workspace, size_t workspace_bytes, dh_stream_t stream);
 
 #ifdef __cplusplus
 }
