@@ -134,9 +134,9 @@ __device__ __forceinline__ void dma16(i32x4 buffer, unsigned voff, unsigned lds)
 
 // One tensor's 64-row tiles through LDS-DMA by NW waves.  Tile row x is token x / group (from the tile's first token on) and head x % group;
 // a key tensor has group 1.
-template <int DP, int NW> struct TileLoader {
+template <int DP, int NW, int ROWS = BN> struct TileLoader {
   using G = Geo<DP>;
-  static constexpr int PER = (BN * G::CH + NW * 64 - 1) / (NW * 64);   // 16-byte chunks a thread
+  static constexpr int PER = (ROWS * G::CH + NW * 64 - 1) / (NW * 64);   // 16-byte chunks a thread
   static constexpr int STEP = NW * 64 / G::CH;                         // rows between two of them
   unsigned voff[PER];
   __device__ __forceinline__ void init(const View& t, int dim, int group, int rows) {
@@ -150,7 +150,7 @@ template <int DP, int NW> struct TileLoader {
   __device__ __forceinline__ void issue(const char* tile, int rows, unsigned lds) const {
     const i32x4 buffer = buffer_at(tile);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = threadIdx.x / G::CH;
-    if (NW * 64 > BN * G::CH && wave * 64 >= BN * G::CH) return;
+    if (NW * 64 > ROWS * G::CH && wave * 64 >= ROWS * G::CH) return;
 #pragma unroll
     for (int i = 0; i < PER; ++i)
       dma16(buffer, r + i * STEP < rows ? voff[i] : OUT_OF_RANGE, lds + (i * NW + wave) * 1024);
@@ -558,28 +558,41 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_dq_kernel(const Params p) {
     }
 }
 
-// dK, dV: one workgroup holds NW x 32 keys of one key head and walks over the rows (tokens x group) that see them, 64 rows a tile.
-// S = Q K^T and dP = dO V^T have one key per lane, so P and dS are B operands of dV^T = dO^T P and dK^T = Q^T dS.
-template <typename T, int DP, int NW>
-__global__ __launch_bounds__(NW * 64, 2) void attn_dkv_kernel(const Params p) {
+// dK, dV: one workgroup holds 128 keys of one key head, 32 a wave, and walks over the rows (tokens x group) that see them, 32 rows a tile.
+// S = Q K^T and dP = dO V^T have one key per lane, so P and dS are B operands of dV^T = dO^T P and dK^T = Q^T dS.  K stays in registers; V
+// does not fit next to the two accumulators (with it the 128-channel form spilled: 6.0 ms instead of the figure below) and is read from LDS.
+// slot >= 0: the walk over the rows is split, 32-bit sums go to the workspace for attn_dkv_join.
+constexpr int DKV_WAVES = 4, DKV_KEYS = DKV_WAVES * 32, DKV_ROWS = 32;
+template <int DP> constexpr int dkv_lds() { return 4 * DKV_ROWS * Geo<DP>::ROWB + DKV_KEYS * Geo<DP>::ROWB + 5 * DKV_ROWS * 4; }
+
+template <typename T, int DP>
+__global__ __launch_bounds__(DKV_WAVES * 64, 2) void attn_dkv_kernel(const Params p) {
   using G = Geo<DP>;
-  extern __shared__ __attribute__((aligned(1024))) char dyn[];               // [buffer][Q, dO], then [buffer][lse2, delta, end][64]
+  constexpr int TB = DKV_ROWS * G::ROWB;
+  extern __shared__ __attribute__((aligned(1024))) char dyn[];               // [buffer][Q, dO], V, [buffer][lse2, delta], tokens of the rows
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const Item it = p.items[blockIdx.x / p.kv_heads];
   const int hk = blockIdx.x % p.kv_heads;
-  if (!item_ok(it, p) || it.first >= it.k_len) return;
+  if (!item_ok(it, p) || it.first >= it.k_len || it.slot >= p.n_slots) return;
   const int key = it.first + wave * 32 + (lane & 31);
   const bool valid = key < it.k_len;
-  u32x4 kf[DP / 16], vf[DP / 16];
+  char* const vtile = dyn + 4 * TB;
+  float* const stat = reinterpret_cast<float*>(vtile + DKV_KEYS * G::ROWB);
+  int* const row_tok = reinterpret_cast<int*>(stat + 4 * DKV_ROWS);
+  lds_char* const lds = (lds_char*)dyn;
+  const unsigned lds0 = (unsigned)(unsigned long)lds;
   {
-    const long r = it.k_start + (valid ? key : it.k_len - 1);
-    const char* kp = p.k.p + r * p.k.st + (long)hk * p.k.sh;
-    const char* vp = p.v.p + r * p.v.st + (long)hk * p.v.sh;
+    TileLoader<DP, DKV_WAVES, DKV_KEYS> l;
+    l.init(p.v, p.dim, 1, DKV_KEYS);
+    l.issue(p.v.p + uniform((long)(it.k_start + it.first) * p.v.st + (long)hk * p.v.sh), it.k_len - it.first, lds0 + 4 * TB);
+  }
+  u32x4 kf[DP / 16];
+  {
+    const char* kp = p.k.p + (long)(it.k_start + (valid ? key : it.k_len - 1)) * p.k.st + (long)hk * p.k.sh;
 #pragma unroll
     for (int s = 0; s < DP / 16; ++s) {
       const int d = 16 * s + 8 * (lane >> 5);
       kf[s] = d < p.dim ? *reinterpret_cast<const u32x4*>(kp + d * 2) : u32x4{0u, 0u, 0u, 0u};
-      vf[s] = d < p.dim ? *reinterpret_cast<const u32x4*>(vp + d * 2) : u32x4{0u, 0u, 0u, 0u};
     }
   }
   f32x16 dk[DP / 32], dv[DP / 32];
@@ -588,109 +601,118 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_dkv_kernel(const Params p) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) dk[mb][i] = dv[mb][i] = 0.f;
 
-  const int tpt = BN / p.group;                                              // tokens a tile
-  TileLoader<DP, NW> lq, lg;
+  const int tpt = DKV_ROWS / p.group;                                        // tokens a tile
+  TileLoader<DP, DKV_WAVES, DKV_ROWS> lq, lg;
   lq.init(p.q, p.dim, p.group, tpt * p.group);
   lg.init(p.g, p.dim, p.group, tpt * p.group);
   const int tok_end = min(it.end, it.q_len);
   const int tiles = (tok_end - it.begin + tpt - 1) / tpt;
   const char* qp = p.q.p + uniform((long)(it.q_start + it.begin) * p.q.st + (long)hk * p.group * p.q.sh);
   const char* gp = p.g.p + uniform((long)(it.q_start + it.begin) * p.g.st + (long)hk * p.group * p.g.sh);
-  lds_char* const lds = (lds_char*)dyn;
-  const unsigned lds0 = (unsigned)(unsigned long)lds;
-  // row statistics of tile t: 64 threads hold a row each
+  // A key is seen from token seen_from(key) on (what keys_seen says, solved for the token): per lane, and for the first and last key of
+  // the wave.
+  auto seen_from = [&](int k) { return p.block ? (int)((unsigned)k / (unsigned)p.block * (unsigned)p.block) - (it.k_len - it.q_len) : 0; };
+  const int from = seen_from(key), wave_any = seen_from(it.first + wave * 32), wave_all = seen_from(min(it.first + wave * 32 + 32, it.k_len) - 1);
+  // row statistics: 32 threads hold a row of the next tile each
   const int mrow = threadIdx.x, mtok = mrow / p.group, mhead = hk * p.group + mrow % p.group;
   float m_lse = INFINITY, m_delta = 0.f;
-  int m_end = 0;
+  if (mrow < DKV_ROWS) row_tok[mrow] = mtok;
   auto fetch = [&](int t) {
-    if (mrow >= BN) return;
+    if (mrow >= DKV_ROWS) return;
     const int tk = it.begin + t * tpt + mtok;
     const bool in = mrow < tpt * p.group && tk < tok_end;
     const long at = (long)(it.q_start + (in ? tk : it.begin)) * p.heads + (in ? mhead : hk * p.group);
     m_lse = in ? p.lse[at] * LOG2E - T::LIFT : INFINITY;                      // p = 0 in rows that do not exist
     m_delta = in ? p.delta[at] : 0.f;
-    m_end = in ? keys_seen(tk, it.q_len, it.k_len, p.block) : 0;
   };
   auto park = [&](int t) {
-    if (mrow >= BN) return;
-    float* f = reinterpret_cast<float*>(dyn + 4 * G::TILEB) + (t & 1) * 3 * BN + mrow;
+    if (mrow >= DKV_ROWS) return;
+    float* f = stat + (t & 1) * 2 * DKV_ROWS + mrow;
     f[0] = m_lse;
-    f[BN] = m_delta;
-    reinterpret_cast<int*>(f)[2 * BN] = m_end;
+    f[DKV_ROWS] = m_delta;
   };
   auto issue = [&](int t) {
-    const unsigned to = lds0 + (t & 1) * 2 * G::TILEB;
-    const int left = min(tok_end - it.begin - t * tpt, tpt) * p.group;
-    lq.issue(qp + (long)t * tpt * p.q.st, left, to);
-    lg.issue(gp + (long)t * tpt * p.g.st, left, to + G::TILEB);
+    const unsigned to = lds0 + (t & 1) * 2 * TB;
+    const int rows = min(tok_end - it.begin - t * tpt, tpt) * p.group;
+    lq.issue(qp + (long)t * tpt * p.q.st, rows, to);
+    lg.issue(gp + (long)t * tpt * p.g.st, rows, to + TB);
   };
   if (tiles > 0) {
     fetch(0);
     issue(0);
     park(0);
   }
-  const int wave_key_end = it.first + wave * 32 + 32;
   for (int t = 0; t < tiles; ++t) {
     DMA_WAIT_BARRIER();
     if (t + 1 < tiles) {
       fetch(t + 1);
       issue(t + 1);
     }
-    const lds_char* qt = lds + (t & 1) * 2 * G::TILEB;
-    const lds_char* gt = qt + G::TILEB;
-    const char* stat = dyn + 4 * G::TILEB + (t & 1) * 3 * BN * 4;
-    const int first_tok = it.begin + t * tpt, last_tok = min(first_tok + tpt, tok_end) - 1;
-    // (ends grow with the token) some row of the tile does not see some key of the wave / no row sees any
-    const bool masked = keys_seen(first_tok, it.q_len, it.k_len, p.block) < wave_key_end;
-    if (keys_seen(last_tok, it.q_len, it.k_len, p.block) > it.first + wave * 32) {
+    const lds_char* qt = lds + (t & 1) * 2 * TB;
+    const lds_char* gt = qt + TB;
+    const lds_char* vt = lds + 4 * TB;
+    const float* st = stat + (t & 1) * 2 * DKV_ROWS;
+    const int first_tok = it.begin + t * tpt;
+    if (first_tok + tpt > wave_any) {                                        // (else no row of the tile sees a key of the wave)
+      f32x16 s, dp;
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        f32x16 s, dp;
+      for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.f;
+      for (int ks = 0; ks < DP / 16; ++ks) {
+        s = T::mfma(frag<DP>(qt, 0, ks, lane), kf[ks], s);
+        dp = T::mfma(frag<DP>(gt, 0, ks, lane), frag<DP>(vt, wave, ks, lane), dp);
+      }
+      const bool masked = first_tok < wave_all;
 #pragma unroll
-        for (int ks = 0; ks < DP / 16; ++ks) {
-          s = T::mfma(frag<DP>(qt, b, ks, lane), kf[ks], s);
-          dp = T::mfma(frag<DP>(gt, b, ks, lane), vf[ks], dp);
+      for (int i4 = 0; i4 < 4; ++i4) {
+        const int r = 8 * i4 + 4 * (lane >> 5);
+        const f32x4 lse2 = *reinterpret_cast<const f32x4*>(st + r);
+        const f32x4 delta = *reinterpret_cast<const f32x4*>(st + DKV_ROWS + r);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int i = 4 * i4 + j;
+          s[i] = exp2_fast(fmaf(s[i], p.c, -lse2[j]));
+          dp[i] = s[i] * (dp[i] - delta[j]);
+        }
+        if (masked) {
+          const i32x4 tok = *reinterpret_cast<const i32x4*>(row_tok + r);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (first_tok + tok[j] < from) s[4 * i4 + j] = dp[4 * i4 + j] = 0.f;
+        }
+      }
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        u32x4 pf, df;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          pf[j] = T::pack(s[8 * ks + 2 * j], s[8 * ks + 2 * j + 1]);
+          df[j] = T::pack(dp[8 * ks + 2 * j], dp[8 * ks + 2 * j + 1]);
         }
 #pragma unroll
-        for (int i4 = 0; i4 < 4; ++i4) {
-          const int r = b * 32 + 8 * i4 + 4 * (lane >> 5);
-          const f32x4 lse2 = *reinterpret_cast<const f32x4*>(stat + r * 4);
-          const f32x4 delta = *reinterpret_cast<const f32x4*>(stat + BN * 4 + r * 4);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int i = 4 * i4 + j;
-            s[i] = exp2_fast(fmaf(s[i], p.c, -lse2[j]));
-            dp[i] = s[i] * (dp[i] - delta[j]);
-          }
-          if (masked) {
-            const i32x4 end = *reinterpret_cast<const i32x4*>(stat + 2 * BN * 4 + r * 4);
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (key >= end[j]) s[4 * i4 + j] = dp[4 * i4 + j] = 0.f;
-          }
-        }
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-          u32x4 pf, df;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            pf[j] = T::pack(s[8 * ks + 2 * j], s[8 * ks + 2 * j + 1]);
-            df[j] = T::pack(dp[8 * ks + 2 * j], dp[8 * ks + 2 * j + 1]);
-          }
-#pragma unroll
-          for (int mb = 0; mb < DP / 32; ++mb) {
-            dv[mb] = T::mfma(frag_t<DP>(gt, b, ks, mb, lane), pf, dv[mb]);
-            dk[mb] = T::mfma(frag_t<DP>(qt, b, ks, mb, lane), df, dk[mb]);
-          }
+        for (int mb = 0; mb < DP / 32; ++mb) {
+          dv[mb] = T::mfma(frag_t<DP>(gt, 0, ks, mb, lane), pf, dv[mb]);
+          dk[mb] = T::mfma(frag_t<DP>(qt, 0, ks, mb, lane), df, dk[mb]);
         }
       }
     }
     if (t + 1 < tiles) park(t + 1);                                          // (its buffer was last read before this iteration's barrier)
   }
-  if (!valid) return;
+  if (tiles == 0) DMA_WAIT_BARRIER();                                        // (V is still on its way)
   const float fv = 1.f / (1 << T::LIFT), fk = p.scale * fv;
+  if (it.slot >= 0) {
+    float* out = p.part + ((((long)it.slot * p.kv_heads + hk) * DKV_KEYS) + wave * 32 + (lane & 31)) * 2 * DP;
+#pragma unroll
+    for (int mb = 0; mb < DP / 32; ++mb)
+#pragma unroll
+      for (int i4 = 0; i4 < 4; ++i4) {
+        const int d = mb * 32 + 8 * i4 + 4 * (lane >> 5);
+        *reinterpret_cast<f32x4*>(out + d) = f32x4{dk[mb][4 * i4] * fk, dk[mb][4 * i4 + 1] * fk, dk[mb][4 * i4 + 2] * fk, dk[mb][4 * i4 + 3] * fk};
+        *reinterpret_cast<f32x4*>(out + DP + d) = f32x4{dv[mb][4 * i4] * fv, dv[mb][4 * i4 + 1] * fv, dv[mb][4 * i4 + 2] * fv, dv[mb][4 * i4 + 3] * fv};
+      }
+    return;
+  }
+  if (!valid) return;
   char* kp = const_cast<char*>(p.dk.p) + (long)(it.k_start + key) * p.dk.st + (long)hk * p.dk.sh;
   char* vp = const_cast<char*>(p.dv.p) + (long)(it.k_start + key) * p.dv.st + (long)hk * p.dv.sh;
 #pragma unroll
@@ -699,18 +721,27 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_dkv_kernel(const Params p) {
     for (int i4 = 0; i4 < 4; ++i4) {
       const int d = mb * 32 + 8 * i4 + 4 * (lane >> 5);
       if (d >= p.dim) continue;
-      u32x2 a, b;
-      a.x = T::pack(dk[mb][4 * i4] * fk, dk[mb][4 * i4 + 1] * fk);
-      a.y = T::pack(dk[mb][4 * i4 + 2] * fk, dk[mb][4 * i4 + 3] * fk);
-      b.x = T::pack(dv[mb][4 * i4] * fv, dv[mb][4 * i4 + 1] * fv);
-      b.y = T::pack(dv[mb][4 * i4 + 2] * fv, dv[mb][4 * i4 + 3] * fv);
-      *reinterpret_cast<u32x2*>(kp + d * 2) = a;
-      *reinterpret_cast<u32x2*>(vp + d * 2) = b;
+      *reinterpret_cast<u32x2*>(kp + d * 2) = u32x2{T::pack(dk[mb][4 * i4] * fk, dk[mb][4 * i4 + 1] * fk), T::pack(dk[mb][4 * i4 + 2] * fk, dk[mb][4 * i4 + 3] * fk)};
+      *reinterpret_cast<u32x2*>(vp + d * 2) = u32x2{T::pack(dv[mb][4 * i4] * fv, dv[mb][4 * i4 + 1] * fv), T::pack(dv[mb][4 * i4 + 2] * fv, dv[mb][4 * i4 + 3] * fv)};
     }
 }
 
+// adds the parts of split keys: items {-, -, k_start, k_len, first, first slot, slots, -}; a thread adds 4 channels of one key
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void attn_dkv_join_kernel(const Params p) {
+  const Item it = p.items[blockIdx.y / p.kv_heads];
+  const int hk = blockIdx.y % p.kv_heads;
+  const int at = blockIdx.x * 256 + threadIdx.x, row = at / (DP / 2), x = at % (DP / 2) * 4;         // x: dK's channels, then dV's
+  const int key = it.first + row, d = x % DP;
+  if (!item_ok(it, p) || key >= it.k_len || d >= p.dim || (long)it.begin + it.end > p.n_slots) return;
+  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < it.end; ++i)
+    sum += *reinterpret_cast<const f32x4*>(p.part + ((((long)(it.begin + i) * p.kv_heads + hk) * DKV_KEYS) + row) * 2 * DP + x);
+  const View& out = x < DP ? p.dk : p.dv;
+  *reinterpret_cast<u32x2*>(const_cast<char*>(out.p) + (long)(it.k_start + key) * out.st + (long)hk * out.sh + d * 2) = u32x2{T::pack(sum.x, sum.y), T::pack(sum.z, sum.w)};
+}
+
 // ---------------------------------------------------------------------------------------------------------------- plan
-constexpr int DKV_WAVES = 4;
 constexpr int SLOTS = 512;                       // workgroups the chip holds at two a CU
 constexpr long MAX_ROWS = 1l << 30;
 
@@ -767,9 +798,13 @@ template <typename T, int DP> int run_bwd(Params p, const dh_attn_info& info, co
   }
   p.items += info.n_dq;
   if (info.n_dkv) {
-    const size_t lds = 4 * Geo<DP>::TILEB + 2 * 3 * BN * 4;
-    DH_LDS_OPTIN((attn_dkv_kernel<T, DP, DKV_WAVES>), lds);
-    hipLaunchKernelGGL((attn_dkv_kernel<T, DP, DKV_WAVES>), dim3((unsigned)(info.n_dkv * info.kv_heads)), dim3(DKV_WAVES * 64), lds, st, p);
+    DH_LDS_OPTIN((attn_dkv_kernel<T, DP>), dkv_lds<DP>());
+    hipLaunchKernelGGL((attn_dkv_kernel<T, DP>), dim3((unsigned)(info.n_dkv * info.kv_heads)), dim3(DKV_WAVES * 64), dkv_lds<DP>(), st, p);
+    DH_LAUNCH_CHECK();
+  }
+  p.items += info.n_dkv;
+  if (info.n_dkv_join) {
+    hipLaunchKernelGGL((attn_dkv_join_kernel<T, DP>), dim3(DKV_KEYS * DP / 2 / 256, (unsigned)(info.n_dkv_join * info.kv_heads)), dim3(256), 0, st, p);
     DH_LAUNCH_CHECK();
   }
   return DH_OK;
@@ -777,8 +812,8 @@ template <typename T, int DP> int run_bwd(Params p, const dh_attn_info& info, co
 
 bool info_ok(const dh_attn_info* i) {
   return i && heads_ok(i->heads, i->kv_heads, i->head_dim) && i->causal_block >= 0 && i->causal_block <= MAX_ROWS && (i->waves == 1 || i->waves == 4 || i->waves == 8) &&
-         i->n_fwd >= 0 && i->n_join >= 0 && i->n_dq >= 0 && i->n_dkv >= 0 && i->n_slots >= 0 && i->q_rows >= 0 && i->k_rows >= 0 && i->q_rows <= MAX_ROWS && i->k_rows <= MAX_ROWS &&
-         i->n_fwd * i->kv_heads <= INT_MAX && i->n_join * i->kv_heads <= 65535 && i->n_dq * i->kv_heads <= INT_MAX && i->n_dkv * i->kv_heads <= INT_MAX;
+         i->n_fwd >= 0 && i->n_join >= 0 && i->n_dq >= 0 && i->n_dkv >= 0 && i->n_dkv_join >= 0 && i->n_slots >= 0 && i->n_dkv_slots >= 0 && i->q_rows >= 0 && i->k_rows >= 0 && i->q_rows <= MAX_ROWS && i->k_rows <= MAX_ROWS &&
+         i->n_fwd * i->kv_heads <= INT_MAX && i->n_join * i->kv_heads <= 65535 && i->n_dq * i->kv_heads <= INT_MAX && i->n_dkv * i->kv_heads <= INT_MAX && i->n_dkv_join * i->kv_heads <= 65535;
 }
 
 }  // namespace
@@ -812,10 +847,20 @@ extern "C" int dh_attn_plan(const int64_t* q_len, const int64_t* k_len, const in
   const long piece = std::max<long>(4, (tiles + SLOTS - 1) / SLOTS);
   Item* base = reinterpret_cast<Item*>(plan);
   const long cap = plan ? plan_ints / 8 : 0;
+  // the same for the rows of dK and dV: a split key tile costs a trip of its sums through memory (a quarter of a millisecond's work for all
+  // of them at most), so pieces are 64 tiles of 32 rows at least
+  long row_tiles = 0;
+  auto rows_of = [&](int64_t i, long x) -> long {              // the first token that sees key x
+    return block ? std::min<long>(q_len[i], std::max<long>(0, x / block * block - (k_len[i] - q_len[i]))) : 0;
+  };
+  const int tpt_k = DKV_ROWS / group;
+  for (int64_t i = 0; i < n_seqs; ++i)
+    for (long x = 0; x < k_len[i]; x += DKV_KEYS) row_tiles += (q_len[i] - rows_of(i, x) + tpt_k - 1) / tpt_k * (long)kv_heads;
+  const long piece_k = std::max<long>(64, (row_tiles + 2 * SLOTS - 1) / (2 * SLOTS));
   Writer w{base, cap, 0};
-  long slots = 0;
-  int64_t counts[4];
-  for (int pass = 0; pass < 4; ++pass) {         // forward items, joins, dQ items, dK / dV items
+  long slots = 0, slots_k = 0;
+  int64_t counts[5];
+  for (int pass = 0; pass < 5; ++pass) {         // forward items, joins, dQ items, dK / dV items, joins
     const long from = w.n;
     long qs = 0, ka = 0, slot = 0;
     for (int64_t i = 0; i < n_seqs; ++i) {
@@ -844,9 +889,25 @@ extern "C" int dh_attn_plan(const int64_t* q_len, const int64_t* k_len, const in
           }
         }
       } else {
-        for (int x = 0; x < n; x += DKV_WAVES * 32) {
-          const long t0 = block ? std::max<long>(0, (long)(x / block) * block - (n - m)) : 0;    // the first token that sees key x
-          w.put(Item{(int)qs, m, ks, n, x, (int)std::min<long>(t0, m), m, -1});
+        for (int x = 0; x < n; x += DKV_KEYS) {
+          const int t0 = (int)rows_of(i, x);
+          Item it{(int)qs, m, ks, n, x, t0, m, -1};
+          const long nt = ((long)m - t0 + tpt_k - 1) / tpt_k;
+          const long pieces = nt > piece_k + piece_k / 2 ? (nt + piece_k - 1) / piece_k : 1;
+          if (pass == 3 && pieces == 1) w.put(it);
+          else if (pass == 3) {
+            for (long y = 0; y < pieces; ++y) {
+              it.begin = (int)(t0 + nt * y / pieces * tpt_k);
+              it.end = (int)std::min<long>(m, t0 + nt * (y + 1) / pieces * tpt_k);
+              it.slot = (int)slot++;
+              w.put(it);
+            }
+          } else if (pieces > 1) {
+            it.begin = (int)slot;
+            it.end = (int)pieces;
+            slot += pieces;
+            w.put(it);
+          }
         }
       }
       qs += m;
@@ -854,9 +915,10 @@ extern "C" int dh_attn_plan(const int64_t* q_len, const int64_t* k_len, const in
       if (slot > INT_MAX || w.n > INT_MAX / 8) return DH_ERR_ARG;
     }
     if (pass == 0) slots = slot;
+    if (pass == 3) slots_k = slot;
     counts[pass] = w.n - from;
     // longest first, so that the last workgroups to start are short ones
-    if (pass != 1 && base && w.n <= cap) std::sort(base + from, base + w.n, longer);
+    if (pass != 1 && pass != 4 && base && w.n <= cap) std::sort(base + from, base + w.n, longer);
   }
   // key ranges of two sequences that share rows: fine to read, but their gradients would be written twice
   bool shared = false;
@@ -874,8 +936,8 @@ extern "C" int dh_attn_plan(const int64_t* q_len, const int64_t* k_len, const in
   info->ints = w.n * 8;
   info->heads = heads; info->kv_heads = kv_heads; info->head_dim = head_dim; info->causal_block = block;
   info->waves = waves;
-  info->n_fwd = counts[0]; info->n_join = counts[1]; info->n_dq = counts[2]; info->n_dkv = counts[3];
-  info->n_slots = slots; info->q_rows = q_rows; info->k_rows = k_rows; info->keys_shared = shared; info->k_total = k_at;
+  info->n_fwd = counts[0]; info->n_join = counts[1]; info->n_dq = counts[2]; info->n_dkv = counts[3]; info->n_dkv_join = counts[4];
+  info->n_slots = slots; info->n_dkv_slots = slots_k; info->q_rows = q_rows; info->k_rows = k_rows; info->keys_shared = shared; info->k_total = k_at;
   if (!info_ok(info)) return DH_ERR_ARG;
   if (plan && plan_ints < info->ints) return DH_ERR_WORKSPACE;
   return DH_OK;
@@ -909,8 +971,10 @@ extern "C" int dh_attn_fwd(const void* q, int64_t q_st, int64_t q_sh, const void
   return dp == 32 ? run_fwd<BF16, 32>(p, *info, items, st) : dp == 64 ? run_fwd<BF16, 64>(p, *info, items, st) : run_fwd<BF16, 128>(p, *info, items, st);
 }
 
+static size_t delta_floats(const dh_attn_info* i) { return ((size_t)i->q_rows * i->heads + 3) / 4 * 4; }
 extern "C" size_t dh_attn_bwd_workspace_bytes(const dh_attn_info* info) {
-  return info_ok(info) ? (size_t)info->q_rows * info->heads * sizeof(float) : 0;
+  if (!info_ok(info)) return 0;
+  return (delta_floats(info) + (size_t)info->n_dkv_slots * info->kv_heads * DKV_KEYS * 2 * pad_dim((int)info->head_dim)) * sizeof(float);
 }
 
 extern "C" int dh_attn_bwd(const void* grad, int64_t g_st, int64_t g_sh, const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh,
@@ -930,11 +994,11 @@ extern "C" int dh_attn_bwd(const void* grad, int64_t g_st, int64_t g_sh, const v
   if (info->n_dq) {
     if (!lse || ((unsigned long)o_low & 15) || !view_ok(p.q, q_rows, info->heads, dim) || !view_ok(p.o, q_rows, info->heads, dim) || !view_ok(p.g, q_rows, info->heads, dim) ||
         !view_ok(p.dq, q_rows, info->heads, dim)) return DH_ERR_ARG;
-    if (!workspace || workspace_bytes < dh_attn_bwd_workspace_bytes(info)) return DH_ERR_WORKSPACE;
+    if (!workspace || ((unsigned long)workspace & 15) || workspace_bytes < dh_attn_bwd_workspace_bytes(info)) return DH_ERR_WORKSPACE;
   }
   if (info->n_dkv && (!view_ok(p.k, k_rows, info->kv_heads, dim) || !view_ok(p.v, k_rows, info->kv_heads, dim) || !view_ok(p.dk, k_rows, info->kv_heads, dim) ||
                       !view_ok(p.dv, k_rows, info->kv_heads, dim))) return DH_ERR_ARG;
-  p.low = (char*)const_cast<void*>(o_low); p.lse = const_cast<float*>(lse); p.delta = (float*)workspace;
+  p.low = (char*)const_cast<void*>(o_low); p.lse = const_cast<float*>(lse); p.delta = (float*)workspace; p.part = (float*)workspace + delta_floats(info); p.n_slots = info->n_dkv_slots;
   p.kv_heads = (int)info->kv_heads; p.heads = (int)info->heads; p.group = p.heads / p.kv_heads; p.dim = dim; p.block = (int)info->causal_block;
   p.q_rows = (int)q_rows; p.k_rows = (int)k_rows; p.scale = scale; p.c = scale * LOG2E;
   const Item* items = reinterpret_cast<const Item*>(plan);

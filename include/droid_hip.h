@@ -495,7 +495,8 @@ typedef struct {
   int64_t ints;                                         /* length of the plan */
   int64_t heads, kv_heads, head_dim, causal_block;
   int64_t waves;                                        /* wavefronts (32 rows each) of a forward workgroup */
-  int64_t n_fwd, n_join, n_dq, n_dkv, n_slots;          /* work items; partial results of split rows */
+  int64_t n_fwd, n_join, n_dq, n_dkv, n_dkv_join;       /* work items */
+  int64_t n_slots, n_dkv_slots;                         /* partial results of split rows / keys, in the workspaces */
   int64_t q_rows, k_rows;                               /* rows that q and k must have at least */
   int64_t k_total;                                      /* sum of k_len */
   int64_t keys_shared;                                  /* two sequences share keys: no backward */
