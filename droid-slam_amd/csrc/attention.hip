@@ -75,6 +75,9 @@ struct BF16 {
   static __device__ __forceinline__ float hi(unsigned u) { return __uint_as_float(u & 0xffff0000u); }
 };
 
+#ifndef FWD64
+#define FWD64 2
+#endif
 constexpr int BN = 64;                           // rows of an LDS tile
 constexpr unsigned OUT_OF_RANGE = 0x80000000u;   // byte offset behind every buffer: such lanes of an LDS-DMA write zeros
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
@@ -130,6 +133,8 @@ __device__ __forceinline__ void dma16(i32x4 buffer, unsigned voff, unsigned lds)
   asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds\n\ts_mov_b32 m0, %0"
                : "=&s"(keep) : "v"(voff), "s"(buffer), "s"(lds) : "memory");
 }
+// keeps a branch a branch: without it the selects of masked tiles are executed (and waited for) in every tile
+#define RARE_BRANCH() asm volatile("")
 #define DMA_WAIT_BARRIER() asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory")
 
 // One tensor's 64-row tiles through LDS-DMA by NW waves.  Tile row x is token x / group (from the tile's first token on) and head x % group;
@@ -250,7 +255,7 @@ template <typename T> __device__ __forceinline__ void add_seen(f32x16& acc, u32x
 // per row; the accumulator is only rescaled when a maximum grew by more than 2^8 (p <= 256 until then: exact in 32 bits, and a 16-bit p
 // keeps its relative precision).  slot >= 0: the row range is split over the keys, unnormalised sums go to the workspace for attn_join.
 template <typename T, int DP, int NW>
-__global__ __launch_bounds__(NW * 64, NW == 1 ? 1 : 2) void attn_fwd_kernel(const Params p) {
+__global__ __launch_bounds__(NW * 64, NW == 1 ? 1 : DP == 128 ? 2 : FWD64) void attn_fwd_kernel(const Params p) {
   using G = Geo<DP>;
   __shared__ __attribute__((aligned(1024))) char smem[4 * G::TILEB];         // [buffer][K, V]
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -316,11 +321,13 @@ __global__ __launch_bounds__(NW * 64, NW == 1 ? 1 : 2) void attn_fwd_kernel(cons
         for (int b = 0; b < 2; ++b) s[b] = T::mfma(frag<DP>(kt, b, ks, lane), qf[ks], s[b]);
       const bool masked = n0 + BN > wmin;
       if (masked) {
+        RARE_BRANCH();
+        const int end = lim - n0 - 4 * (lane >> 5);
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
           for (int i = 0; i < 16; ++i)
-            if (n0 + b * 32 + 8 * (i / 4) + 4 * (lane >> 5) + (i & 3) >= lim) s[b][i] = -INFINITY;
+            if (b * 32 + 8 * (i / 4) + (i & 3) >= end) s[b][i] = -INFINITY;
       }
       float mx = s[0][0];
 #pragma unroll
@@ -529,9 +536,11 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_dq_kernel(const Params p) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[i] = exp2_fast(fmaf(s[i], p.c, -lse2)) * (dp[i] - delta);
       if (masked) {
+        RARE_BRANCH();
+        const int end = lim - n0 - 4 * (lane >> 5);
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-          if (n0 + b * 32 + 8 * (i / 4) + 4 * (lane >> 5) + (i & 3) >= lim) s[i] = 0.f;
+          if (b * 32 + 8 * (i / 4) + (i & 3) >= end) s[i] = 0.f;
       }
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks) {
@@ -558,19 +567,24 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_dq_kernel(const Params p) {
     }
 }
 
-// dK, dV: one workgroup holds 128 keys of one key head, 32 a wave, and walks over the rows (tokens x group) that see them, 32 rows a tile.
+// dK, dV: one workgroup holds 128 keys of one key head (64 where head_dim <= 64: half as long a walk, see below), 32 a wave, and walks over the
+// rows (tokens x group) that see them, 32 (64, in two waves) rows a tile.
 // S = Q K^T and dP = dO V^T have one key per lane, so P and dS are B operands of dV^T = dO^T P and dK^T = Q^T dS.  K stays in registers; V
 // does not fit next to the two accumulators (with it the 128-channel form spilled: 6.0 ms instead of the figure below) and is read from LDS.
 // slot >= 0: the walk over the rows is split, 32-bit sums go to the workspace for attn_dkv_join.
-constexpr int DKV_WAVES = 4, DKV_KEYS = DKV_WAVES * 32, DKV_ROWS = 32;
-template <int DP> constexpr int dkv_lds() { return 4 * DKV_ROWS * Geo<DP>::ROWB + DKV_KEYS * Geo<DP>::ROWB + 5 * DKV_ROWS * 4; }
+constexpr int DKV_WAVES = 4;
+template <int DP> struct Dkv {
+  static constexpr int KW = DP == 128 ? 4 : 2, RW = DKV_WAVES / KW;          // waves along the keys / along the rows
+  static constexpr int KEYS = KW * 32, ROWS = RW * 32, TB = ROWS * Geo<DP>::ROWB;
+  static constexpr int LDS = 4 * TB + KEYS * Geo<DP>::ROWB + 5 * ROWS * 4;
+};
 
 template <typename T, int DP>
-__global__ __launch_bounds__(DKV_WAVES * 64, 2) void attn_dkv_kernel(const Params p) {
+__global__ __launch_bounds__(DKV_WAVES * 64, DP == 128 ? 2 : 3) void attn_dkv_kernel(const Params p) {
   using G = Geo<DP>;
-  constexpr int TB = DKV_ROWS * G::ROWB;
+  constexpr int TB = Dkv<DP>::TB, DKV_ROWS = Dkv<DP>::ROWS, DKV_KEYS = Dkv<DP>::KEYS;
   extern __shared__ __attribute__((aligned(1024))) char dyn[];               // [buffer][Q, dO], V, [buffer][lse2, delta], tokens of the rows
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = (threadIdx.x >> 6) % Dkv<DP>::KW, rw = (threadIdx.x >> 6) / Dkv<DP>::KW;       // 32 keys, 32 rows of a tile
   const Item it = p.items[blockIdx.x / p.kv_heads];
   const int hk = blockIdx.x % p.kv_heads;
   if (!item_ok(it, p) || it.first >= it.k_len || it.slot >= p.n_slots) return;
@@ -659,13 +673,13 @@ __global__ __launch_bounds__(DKV_WAVES * 64, 2) void attn_dkv_kernel(const Param
       for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.f;
 #pragma unroll
       for (int ks = 0; ks < DP / 16; ++ks) {
-        s = T::mfma(frag<DP>(qt, 0, ks, lane), kf[ks], s);
-        dp = T::mfma(frag<DP>(gt, 0, ks, lane), frag<DP>(vt, wave, ks, lane), dp);
+        s = T::mfma(frag<DP>(qt, rw, ks, lane), kf[ks], s);
+        dp = T::mfma(frag<DP>(gt, rw, ks, lane), frag<DP>(vt, wave, ks, lane), dp);
       }
       const bool masked = first_tok < wave_all;
 #pragma unroll
       for (int i4 = 0; i4 < 4; ++i4) {
-        const int r = 8 * i4 + 4 * (lane >> 5);
+        const int r = rw * 32 + 8 * i4 + 4 * (lane >> 5);
         const f32x4 lse2 = *reinterpret_cast<const f32x4*>(st + r);
         const f32x4 delta = *reinterpret_cast<const f32x4*>(st + DKV_ROWS + r);
 #pragma unroll
@@ -675,6 +689,7 @@ __global__ __launch_bounds__(DKV_WAVES * 64, 2) void attn_dkv_kernel(const Param
           dp[i] = s[i] * (dp[i] - delta[j]);
         }
         if (masked) {
+          RARE_BRANCH();
           const i32x4 tok = *reinterpret_cast<const i32x4*>(row_tok + r);
 #pragma unroll
           for (int j = 0; j < 4; ++j)
@@ -691,14 +706,30 @@ __global__ __launch_bounds__(DKV_WAVES * 64, 2) void attn_dkv_kernel(const Param
         }
 #pragma unroll
         for (int mb = 0; mb < DP / 32; ++mb) {
-          dv[mb] = T::mfma(frag_t<DP>(gt, 0, ks, mb, lane), pf, dv[mb]);
-          dk[mb] = T::mfma(frag_t<DP>(qt, 0, ks, mb, lane), df, dk[mb]);
+          dv[mb] = T::mfma(frag_t<DP>(gt, rw, ks, mb, lane), pf, dv[mb]);
+          dk[mb] = T::mfma(frag_t<DP>(qt, rw, ks, mb, lane), df, dk[mb]);
         }
       }
     }
     if (t + 1 < tiles) park(t + 1);                                          // (its buffer was last read before this iteration's barrier)
   }
   if (tiles == 0) DMA_WAIT_BARRIER();                                        // (V is still on its way)
+  if constexpr (Dkv<DP>::RW == 2) {                                          // the two halves of the rows meet in LDS, where the tiles were
+    float* sum = reinterpret_cast<float*>(dyn) + wave * (DP * 64) + lane;
+    __syncthreads();
+    if (rw) {
+#pragma unroll
+      for (int mb = 0; mb < DP / 32; ++mb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) { sum[(mb * 32 + i) * 64] = dk[mb][i]; sum[(mb * 32 + 16 + i) * 64] = dv[mb][i]; }
+    }
+    __syncthreads();
+    if (rw) return;
+#pragma unroll
+    for (int mb = 0; mb < DP / 32; ++mb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) { dk[mb][i] += sum[(mb * 32 + i) * 64]; dv[mb][i] += sum[(mb * 32 + 16 + i) * 64]; }
+  }
   const float fv = 1.f / (1 << T::LIFT), fk = p.scale * fv;
   if (it.slot >= 0) {
     float* out = p.part + ((((long)it.slot * p.kv_heads + hk) * DKV_KEYS) + wave * 32 + (lane & 31)) * 2 * DP;
@@ -736,7 +767,7 @@ __global__ __launch_bounds__(256) void attn_dkv_join_kernel(const Params p) {
   if (!item_ok(it, p) || key >= it.k_len || d >= p.dim || (long)it.begin + it.end > p.n_slots) return;
   f32x4 sum = {0.f, 0.f, 0.f, 0.f};
   for (int i = 0; i < it.end; ++i)
-    sum += *reinterpret_cast<const f32x4*>(p.part + ((((long)(it.begin + i) * p.kv_heads + hk) * DKV_KEYS) + row) * 2 * DP + x);
+    sum += *reinterpret_cast<const f32x4*>(p.part + ((((long)(it.begin + i) * p.kv_heads + hk) * Dkv<DP>::KEYS) + row) * 2 * DP + x);
   const View& out = x < DP ? p.dk : p.dv;
   *reinterpret_cast<u32x2*>(const_cast<char*>(out.p) + (long)(it.k_start + key) * out.st + (long)hk * out.sh + d * 2) = u32x2{T::pack(sum.x, sum.y), T::pack(sum.z, sum.w)};
 }
@@ -798,13 +829,13 @@ template <typename T, int DP> int run_bwd(Params p, const dh_attn_info& info, co
   }
   p.items += info.n_dq;
   if (info.n_dkv) {
-    DH_LDS_OPTIN((attn_dkv_kernel<T, DP>), dkv_lds<DP>());
-    hipLaunchKernelGGL((attn_dkv_kernel<T, DP>), dim3((unsigned)(info.n_dkv * info.kv_heads)), dim3(DKV_WAVES * 64), dkv_lds<DP>(), st, p);
+    DH_LDS_OPTIN((attn_dkv_kernel<T, DP>), Dkv<DP>::LDS);
+    hipLaunchKernelGGL((attn_dkv_kernel<T, DP>), dim3((unsigned)(info.n_dkv * info.kv_heads)), dim3(DKV_WAVES * 64), Dkv<DP>::LDS, st, p);
     DH_LAUNCH_CHECK();
   }
   p.items += info.n_dkv;
   if (info.n_dkv_join) {
-    hipLaunchKernelGGL((attn_dkv_join_kernel<T, DP>), dim3(DKV_KEYS * DP / 2 / 256, (unsigned)(info.n_dkv_join * info.kv_heads)), dim3(256), 0, st, p);
+    hipLaunchKernelGGL((attn_dkv_join_kernel<T, DP>), dim3(Dkv<DP>::KEYS * DP / 2 / 256, (unsigned)(info.n_dkv_join * info.kv_heads)), dim3(256), 0, st, p);
     DH_LAUNCH_CHECK();
   }
   return DH_OK;
@@ -853,9 +884,10 @@ extern "C" int dh_attn_plan(const int64_t* q_len, const int64_t* k_len, const in
   auto rows_of = [&](int64_t i, long x) -> long {              // the first token that sees key x
     return block ? std::min<long>(q_len[i], std::max<long>(0, x / block * block - (k_len[i] - q_len[i]))) : 0;
   };
-  const int tpt_k = DKV_ROWS / group;
+  const bool wide = pad_dim(head_dim) == 128;
+  const int dkv_keys = wide ? Dkv<128>::KEYS : Dkv<64>::KEYS, tpt_k = (wide ? Dkv<128>::ROWS : Dkv<64>::ROWS) / group;
   for (int64_t i = 0; i < n_seqs; ++i)
-    for (long x = 0; x < k_len[i]; x += DKV_KEYS) row_tiles += (q_len[i] - rows_of(i, x) + tpt_k - 1) / tpt_k * (long)kv_heads;
+    for (long x = 0; x < k_len[i]; x += dkv_keys) row_tiles += (q_len[i] - rows_of(i, x) + tpt_k - 1) / tpt_k * (long)kv_heads;
   const long piece_k = std::max<long>(64, (row_tiles + 2 * SLOTS - 1) / (2 * SLOTS));
   Writer w{base, cap, 0};
   long slots = 0, slots_k = 0;
@@ -889,7 +921,7 @@ extern "C" int dh_attn_plan(const int64_t* q_len, const int64_t* k_len, const in
           }
         }
       } else {
-        for (int x = 0; x < n; x += DKV_KEYS) {
+        for (int x = 0; x < n; x += dkv_keys) {
           const int t0 = (int)rows_of(i, x);
           Item it{(int)qs, m, ks, n, x, t0, m, -1};
           const long nt = ((long)m - t0 + tpt_k - 1) / tpt_k;
@@ -974,7 +1006,7 @@ extern "C" int dh_attn_fwd(const void* q, int64_t q_st, int64_t q_sh, const void
 static size_t delta_floats(const dh_attn_info* i) { return ((size_t)i->q_rows * i->heads + 3) / 4 * 4; }
 extern "C" size_t dh_attn_bwd_workspace_bytes(const dh_attn_info* info) {
   if (!info_ok(info)) return 0;
-  return (delta_floats(info) + (size_t)info->n_dkv_slots * info->kv_heads * DKV_KEYS * 2 * pad_dim((int)info->head_dim)) * sizeof(float);
+  return (delta_floats(info) + (size_t)info->n_dkv_slots * info->kv_heads * (pad_dim((int)info->head_dim) == 128 ? Dkv<128>::KEYS : Dkv<64>::KEYS) * 2 * pad_dim((int)info->head_dim)) * sizeof(float);
 }
 
 extern "C" int dh_attn_bwd(const void* grad, int64_t g_st, int64_t g_sh, const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh,

@@ -54,7 +54,7 @@ def test_plan_covers_every_row_and_key_once(lengths, key_lengths, heads, kv_head
         for qs, ql, ks, kl, first, begin, end, _ in dkv:
             if (qs, ql) == (q0, m) and (ks, kl) == (k0, l) and l:
                 assert 0 <= begin <= end <= m
-                hit[begin:end, first:first + 128] += 1
+                hit[begin:end, first:first + 64] += 1
         assert bool((hit[seen] == 1).all()) and bool((hit <= 1).all())
         q0, k0 = q0 + m, k0 + l
     slots = sorted(x for j in join for x in range(j[5], j[5] + j[6]))
