@@ -75,9 +75,6 @@ struct BF16 {
   static __device__ __forceinline__ float hi(unsigned u) { return __uint_as_float(u & 0xffff0000u); }
 };
 
-#ifndef FWD64
-#define FWD64 2
-#endif
 constexpr int BN = 64;                           // rows of an LDS tile
 constexpr unsigned OUT_OF_RANGE = 0x80000000u;   // byte offset behind every buffer: such lanes of an LDS-DMA write zeros
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
@@ -135,6 +132,11 @@ __device__ __forceinline__ void dma16(i32x4 buffer, unsigned voff, unsigned lds)
 }
 // keeps a branch a branch: without it the selects of masked tiles are executed (and waited for) in every tile
 #define RARE_BRANCH() asm volatile("")
+// all but the last `LEFT` DMA instructions of this wave have arrived
+template <int LEFT, bool BARRIER> __device__ __forceinline__ void dma_wait() {
+  if constexpr (BARRIER) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LEFT) : "memory");
+  else asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LEFT) : "memory");
+}
 #define DMA_WAIT_BARRIER() asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory")
 
 // One tensor's 64-row tiles through LDS-DMA by NW waves.  Tile row x is token x / group (from the tile's first token on) and head x % group;
@@ -254,10 +256,15 @@ template <typename T> __device__ __forceinline__ void add_seen(f32x16& acc, u32x
 // One workgroup: NW x 32 rows (NW * 32 / group tokens) of one key head over the keys [begin, end) of its sequence.  Running maximum and sum
 // per row; the accumulator is only rescaled when a maximum grew by more than 2^8 (p <= 256 until then: exact in 32 bits, and a 16-bit p
 // keeps its relative precision).  slot >= 0: the row range is split over the keys, unnormalised sums go to the workspace for attn_join.
+// How the keys come in: 64 keys a tile, one tile ahead; a lone wave (few rows, bound by memory) takes 32 and keeps two
+// tiles on their way in 48 KB, three waves a CU (32 queries over 358 MB of keys: 90 us; two or four stages with as many waves as fit 99 and 95).
+template <int NW> struct Walk { static constexpr int BLOCKS = NW == 1 ? 1 : 2, STAGES = NW == 1 ? 3 : 2; };
+
 template <typename T, int DP, int NW>
-__global__ __launch_bounds__(NW * 64, NW == 1 ? 1 : DP == 128 ? 2 : FWD64) void attn_fwd_kernel(const Params p) {
+__global__ __launch_bounds__(NW * 64, NW == 1 ? 1 : DP == 128 ? 2 : 3) void attn_fwd_kernel(const Params p) {
   using G = Geo<DP>;
-  __shared__ __attribute__((aligned(1024))) char smem[4 * G::TILEB];         // [buffer][K, V]
+  constexpr int KB = Walk<NW>::BLOCKS, TK = KB * 32, ST = Walk<NW>::STAGES, TB = TK * G::ROWB;
+  __shared__ __attribute__((aligned(1024))) char smem[ST * 2 * TB];          // [stage][K, V]
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const Item it = p.items[blockIdx.x / p.kv_heads];
   const int hk = blockIdx.x % p.kv_heads;
@@ -280,19 +287,19 @@ __global__ __launch_bounds__(NW * 64, NW == 1 ? 1 : DP == 128 ? 2 : FWD64) void 
   }
   f32x16 acc[DP / 32];
   float m, l;                                                                // l: this half's keys only
-  TileLoader<DP, NW> lk, lv;
-  lk.init(p.k, p.dim, 1, BN);
-  lv.init(p.v, p.dim, 1, BN);
+  TileLoader<DP, NW, TK> lk, lv;
+  lk.init(p.k, p.dim, 1, TK);
+  lv.init(p.v, p.dim, 1, TK);
   const char* kp = p.k.p + uniform((long)(it.k_start + it.begin) * p.k.st + (long)hk * p.k.sh);
   const char* vp = p.v.p + uniform((long)(it.k_start + it.begin) * p.v.st + (long)hk * p.v.sh);
   lds_char* const lds = (lds_char*)smem;
   const unsigned lds0 = (unsigned)(unsigned long)lds;
-  const int tiles = (key_end - it.begin + BN - 1) / BN;
+  const int tiles = (key_end - it.begin + TK - 1) / TK;
   auto issue = [&](int t) {
-    const unsigned to = lds0 + (t & 1) * 2 * G::TILEB;
-    const int left = key_end - it.begin - t * BN;
-    lk.issue(kp + (long)t * BN * p.k.st, left, to);
-    lv.issue(vp + (long)t * BN * p.v.st, left, to + G::TILEB);
+    const unsigned to = lds0 + t % ST * 2 * TB;
+    const int left = key_end - it.begin - t * TK;                            // (behind the last tile: nothing, zeros go to a stage nobody reads)
+    lk.issue(kp + (long)t * TK * p.k.st, left, to);
+    lv.issue(vp + (long)t * TK * p.v.st, left, to + TB);
   };
   auto walk = [&](auto careful) {
     constexpr bool CAREFUL = decltype(careful)::value;
@@ -302,38 +309,39 @@ __global__ __launch_bounds__(NW * 64, NW == 1 ? 1 : DP == 128 ? 2 : FWD64) void 
     for (int mb = 0; mb < DP / 32; ++mb)
 #pragma unroll
       for (int i = 0; i < 16; ++i) acc[mb][i] = 0.f;
-    if (tiles > 0) issue(0);
+    for (int t = 0; t < ST - 1; ++t) issue(t);
     for (int t = 0; t < tiles; ++t) {
-      DMA_WAIT_BARRIER();                                                      // tile t is there, and everybody has left tile t - 1
-      if (t + 1 < tiles) issue(t + 1);
-      const int n0 = it.begin + t * BN;
+      // tile t is there (the stages behind it may still be on their way), and everybody has left tile t - 1
+      dma_wait<(ST - 2) * 2 * TileLoader<DP, NW, TK>::PER, (NW > 1)>();
+      issue(t + ST - 1);
+      const int n0 = it.begin + t * TK;
       if (n0 >= wmax) continue;
-      const lds_char* kt = lds + (t & 1) * 2 * G::TILEB;
-      const lds_char* vt = kt + G::TILEB;
-      f32x16 s[2];
+      const lds_char* kt = lds + t % ST * 2 * TB;
+      const lds_char* vt = kt + TB;
+      f32x16 s[KB];
 #pragma unroll
-      for (int b = 0; b < 2; ++b)
+      for (int b = 0; b < KB; ++b)
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[b][i] = 0.f;
 #pragma unroll
       for (int ks = 0; ks < DP / 16; ++ks)
 #pragma unroll
-        for (int b = 0; b < 2; ++b) s[b] = T::mfma(frag<DP>(kt, b, ks, lane), qf[ks], s[b]);
-      const bool masked = n0 + BN > wmin;
+        for (int b = 0; b < KB; ++b) s[b] = T::mfma(frag<DP>(kt, b, ks, lane), qf[ks], s[b]);
+      const bool masked = n0 + TK > wmin;
       if (masked) {
         RARE_BRANCH();
         const int end = lim - n0 - 4 * (lane >> 5);
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
+        for (int b = 0; b < KB; ++b)
 #pragma unroll
           for (int i = 0; i < 16; ++i)
             if (b * 32 + 8 * (i / 4) + (i & 3) >= end) s[b][i] = -INFINITY;
       }
       float mx = s[0][0];
 #pragma unroll
-      for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[0][i]);
+      for (int b = 0; b < KB; ++b)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[1][i]);
+        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[b][i]);
       mx = fmaxf(mx, other_half(mx)) * p.c;
       if (__any(mx > m + 8.f)) {
         const float mn = mx > m + 8.f ? mx : m, a = exp2_fast(m - mn);       // (a row's bits do not depend on its neighbours)
@@ -344,9 +352,9 @@ __global__ __launch_bounds__(NW * 64, NW == 1 ? 1 : DP == 128 ? 2 : FWD64) void 
 #pragma unroll
           for (int i = 0; i < 16; ++i) acc[mb][i] *= a;
       }
-      u32x4 pf[2][2];
+      u32x4 pf[KB][2];
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
+      for (int b = 0; b < KB; ++b) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           s[b][i] = exp2_fast(fmaf(s[b][i], p.c, -m));
@@ -358,7 +366,7 @@ __global__ __launch_bounds__(NW * 64, NW == 1 ? 1 : DP == 128 ? 2 : FWD64) void 
           for (int j = 0; j < 4; ++j) pf[b][ks][j] = T::pack(s[b][8 * ks + 2 * j], s[b][8 * ks + 2 * j + 1]);
       }
 #pragma unroll
-      for (int b = 0; b < 2; ++b)
+      for (int b = 0; b < KB; ++b)
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
@@ -368,6 +376,7 @@ __global__ __launch_bounds__(NW * 64, NW == 1 ? 1 : DP == 128 ? 2 : FWD64) void 
             else acc[mb] = T::mfma(vf, pf[b][ks], acc[mb]);
           }
     }
+    dma_wait<0, false>();
   };
   walk(std::false_type());
   // A value that is not finite makes 0 * v of the rows that do not see it NaN.  Only then the workgroup walks a second time.
@@ -433,20 +442,38 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const Params p, int rows
   const int hk = blockIdx.y % p.kv_heads;
   const int row = blockIdx.x * 8 + threadIdx.x / 32, x = threadIdx.x & 31;
   const int tok = it.first + row / p.group, head = hk * p.group + row % p.group;
-  if (row >= rows / p.group * p.group || tok >= it.q_len || !item_ok(it, p) || (long)it.begin + it.end > p.n_slots) return;
+  if (row >= rows / p.group * p.group || tok >= it.q_len || !item_ok(it, p) || (long)it.begin + it.end > p.n_slots) return;   // (whole halves of waves)
+  // lane x holds the statistics of part x (x + 32, ...); all loads of a loop are independent of each other
   const float* pm = p.part + p.n_slots * p.kv_heads * rows * DP;
-  float m = M_FLOOR;
-  for (int i = 0; i < it.end; ++i) m = fmaxf(m, pm[(((long)(it.begin + i) * p.kv_heads + hk) * rows + row) * 2]);
-  float l = 0.f, acc[DP / 32];
+  const auto at = [&](int i) { return ((long)(it.begin + i) * p.kv_heads + hk) * rows + row; };
+  float m = M_FLOOR, l = 0.f, acc[DP / 32];
+  for (int i = x; i < it.end; i += 32) m = fmaxf(m, pm[at(i) * 2]);
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
 #pragma unroll
   for (int k = 0; k < DP / 32; ++k) acc[k] = 0.f;
-  for (int i = 0; i < it.end; ++i) {
-    const long at = ((long)(it.begin + i) * p.kv_heads + hk) * rows + row;
-    const float a = exp2f(pm[at * 2] - m);
-    l += a * pm[at * 2 + 1];
+  for (int i0 = 0; i0 < it.end; i0 += 32) {
+    const int n = min(32, it.end - i0);
+    const float w = x < n ? exp2f(pm[at(i0 + x) * 2] - m) : 0.f;
+    if (x < n) l += w * pm[at(i0 + x) * 2 + 1];
+    for (int j0 = 0; j0 < n; j0 += 8) {
+      float v[8][DP / 32];
 #pragma unroll
-    for (int k = 0; k < DP / 32; ++k) acc[k] += a * p.part[at * DP + k * 32 + x];
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int k = 0; k < DP / 32; ++k) v[j][k] = p.part[at(i0 + min(j0 + j, n - 1)) * DP + k * 32 + x];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float a = __shfl(w, (threadIdx.x & 32) + j0 + j, 64);          // (0 from n on)
+        if (j0 + j < n) {
+#pragma unroll
+          for (int k = 0; k < DP / 32; ++k) acc[k] += a * v[j][k];
+        }
+      }
+    }
   }
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) l += __shfl_xor(l, off, 64);
   const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
   unsigned short* op = reinterpret_cast<unsigned short*>(const_cast<char*>(p.o.p) + (long)(it.q_start + tok) * p.o.st + (long)head * p.o.sh);
 #pragma unroll
@@ -773,7 +800,6 @@ __global__ __launch_bounds__(256) void attn_dkv_join_kernel(const Params p) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------- plan
-constexpr int SLOTS = 512;                       // workgroups the chip holds at two a CU
 constexpr long MAX_ROWS = 1l << 30;
 
 int pad_dim(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
@@ -867,17 +893,26 @@ extern "C" int dh_attn_plan(const int64_t* q_len, const int64_t* k_len, const in
   // rows a workgroup: one wave where a tile of 32 holds every row of the longest sequence (decoding), else 128
   const int waves = most * group <= 32 ? 1 : 4;
   const int tpt = waves * 32 / group, tpt_q = 128 / group;
-  long tiles = 0;                                // key tiles of all rows: what there is to spread
-  for (int64_t i = 0; i < n_seqs; ++i)
-    for (long t = 0; t < q_len[i]; t += tpt) {
-      const int e = keys_seen((int)std::min<long>(q_len[i], t + tpt) - 1, (int)q_len[i], (int)k_len[i], block);
-      tiles += (e + BN - 1) / BN * (long)kv_heads;
+  // Long walks over the keys become several work items (pieces of whole key tiles, joined afterwards) where they would outlast the rest:
+  // the aim is an equal share of all key tiles for each of the workgroups that the chip holds at once.  A walk is only split if that saves
+  // 8 tiles: a split row's sums go through memory once more, and the join is a launch of its own.
+  const int dp = pad_dim(head_dim), slots_on_chip = 256 * (waves == 1 ? (dp == 128 ? 3 : 6) : dp == 128 ? 2 : 3);       // LDS or registers hold no more
+  const int64_t* ql = q_len; const int64_t* kl = k_len;
+  auto each_tile = [&](auto&& f) {
+    for (int64_t i = 0; i < n_seqs; ++i)
+      for (long t = 0; t < ql[i]; t += tpt) f((keys_seen((int)std::min<long>(ql[i], t + tpt) - 1, (int)ql[i], (int)kl[i], block) + BN - 1) / BN);
+  };
+  long tiles = 0, walks = 0;
+  each_tile([&](long nt) { tiles += nt * kv_heads; walks += kv_heads; });
+  long piece = std::max<long>(4, (tiles + slots_on_chip - 1) / slots_on_chip);
+  auto pieces_of = [&](long nt) -> long { return nt > piece + piece / 8 + 8 ? (nt + piece - 1) / piece : 1; };
+  if (walks < slots_on_chip)                     // rounding up must not leave a few items for a second round
+    for (;;) {
+      long n = 0, longest = 0;
+      each_tile([&](long nt) { n += pieces_of(nt) * kv_heads; longest = std::max(longest, nt); });
+      if (n <= slots_on_chip || longest <= piece) break;
+      piece += std::max<long>(1, piece / 16);
     }
-  // few rows over many keys: ranges of keys become work items of their own.  At least 4 tiles each, and only where there is less than one
-  // item for each place on the chip.
-  const long piece = std::max<long>(4, (tiles + SLOTS - 1) / SLOTS);
-  Item* base = reinterpret_cast<Item*>(plan);
-  const long cap = plan ? plan_ints / 8 : 0;
   // the same for the rows of dK and dV: a split key tile costs a trip of its sums through memory (a quarter of a millisecond's work for all
   // of them at most), so pieces are 64 tiles of 32 rows at least
   long row_tiles = 0;
@@ -888,7 +923,9 @@ extern "C" int dh_attn_plan(const int64_t* q_len, const int64_t* k_len, const in
   const int dkv_keys = wide ? Dkv<128>::KEYS : Dkv<64>::KEYS, tpt_k = (wide ? Dkv<128>::ROWS : Dkv<64>::ROWS) / group;
   for (int64_t i = 0; i < n_seqs; ++i)
     for (long x = 0; x < k_len[i]; x += dkv_keys) row_tiles += (q_len[i] - rows_of(i, x) + tpt_k - 1) / tpt_k * (long)kv_heads;
-  const long piece_k = std::max<long>(64, (row_tiles + 2 * SLOTS - 1) / (2 * SLOTS));
+  const long piece_k = std::max<long>(64, (row_tiles + 1023) / 1024);
+  Item* base = reinterpret_cast<Item*>(plan);
+  const long cap = plan ? plan_ints / 8 : 0;
   Writer w{base, cap, 0};
   long slots = 0, slots_k = 0;
   int64_t counts[5];
@@ -904,7 +941,7 @@ extern "C" int dh_attn_plan(const int64_t* q_len, const int64_t* k_len, const in
           const int e = keys_seen(std::min(m, t + step) - 1, m, n, block);
           Item it{(int)qs, m, ks, n, t, 0, e, -1};
           const long nt = (e + BN - 1) / BN;
-          const long pieces = nt > piece + piece / 2 ? (nt + piece - 1) / piece : 1;
+          const long pieces = pieces_of(nt);
           if (pass == 2 || (pass == 0 && pieces == 1)) w.put(it);
           else if (pass == 0) {
             for (long x = 0; x < pieces; ++x) {
