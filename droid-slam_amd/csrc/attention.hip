@@ -93,6 +93,7 @@ struct Params {
   float* part;                                   // split rows: [slot, kv_heads, rows, DP] and behind them [slot, kv_heads, rows, 2]
   const Item* items;
   long n_slots;
+  int blocks, clear_q, clear_k;                  // workgroups of work items; from there on: rows [clear_q, q_rows) / [clear_k, k_rows) are cleared
   int kv_heads, group, heads, dim, block, q_rows, k_rows;
   float c;                                       // scale * log2(e)
   float scale;
@@ -252,6 +253,16 @@ template <typename T> __device__ __forceinline__ void add_seen(f32x16& acc, u32x
   }
 }
 
+// workgroups behind the work items: rows [from, to) of a dense or strided result become zero
+template <int THREADS> __device__ __forceinline__ void clear_rows(const View& t, int from, int to, int heads, int dim, int part, int parts) {
+  const long n = (long)(to - from) * heads * (dim / 8);
+  for (long i = (long)part * THREADS + threadIdx.x; i < n; i += (long)parts * THREADS) {
+    const long c = i % (dim / 8), r = i / (dim / 8);
+    *reinterpret_cast<u32x4*>(const_cast<char*>(t.p) + (from + r / heads) * t.st + r % heads * t.sh + c * 16) = u32x4{0u, 0u, 0u, 0u};
+  }
+}
+constexpr int CLEAR_BYTES = 1 << 15;             // a workgroup's share
+
 // ------------------------------------------------------------------------------------------------------------- forward
 // One workgroup: NW x 32 rows (NW * 32 / group tokens) of one key head over the keys [begin, end) of its sequence.  Running maximum and sum
 // per row; the accumulator is only rescaled when a maximum grew by more than 2^8 (p <= 256 until then: exact in 32 bits, and a 16-bit p
@@ -266,6 +277,12 @@ __global__ __launch_bounds__(NW * 64, NW == 1 ? 1 : DP == 128 ? 2 : 3) void attn
   constexpr int KB = Walk<NW>::BLOCKS, TK = KB * 32, ST = Walk<NW>::STAGES, TB = TK * G::ROWB;
   __shared__ __attribute__((aligned(1024))) char smem[ST * 2 * TB];          // [stage][K, V]
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (blockIdx.x >= p.blocks) {
+    const int part = blockIdx.x - p.blocks, parts = gridDim.x - p.blocks;
+    clear_rows<NW * 64>(p.o, p.clear_q, p.q_rows, p.heads, p.dim, part, parts);
+    for (long i = (long)p.clear_q * p.heads + part * NW * 64 + threadIdx.x; i < (long)p.q_rows * p.heads; i += parts * NW * 64) p.lse[i] = -INFINITY;
+    return;
+  }
   const Item it = p.items[blockIdx.x / p.kv_heads];
   const int hk = blockIdx.x % p.kv_heads;
   if (!item_ok(it, p) || it.first >= it.q_len || it.slot >= p.n_slots) return;
@@ -494,9 +511,13 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_dq_kernel(const Params p) {
   using G = Geo<DP>;
   __shared__ __attribute__((aligned(1024))) char smem[4 * G::TILEB];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (blockIdx.x >= p.blocks) {
+    clear_rows<NW * 64>(p.dq, p.clear_q, p.q_rows, p.heads, p.dim, blockIdx.x - p.blocks, gridDim.x - p.blocks);
+    return;
+  }
   const Item it = p.items[blockIdx.x / p.kv_heads];
   const int hk = blockIdx.x % p.kv_heads;
-  if (!item_ok(it, p) || it.first >= it.q_len || it.slot >= p.n_slots) return;
+  if (!item_ok(it, p) || it.first >= it.q_len) return;
   const int row = wave * 32 + (lane & 31), tpt = NW * 32 / p.group;
   const int tok = it.first + row / p.group, head = hk * p.group + row % p.group;
   const bool valid = row < tpt * p.group && tok < it.q_len;
@@ -612,6 +633,11 @@ __global__ __launch_bounds__(DKV_WAVES * 64, DP == 128 ? 2 : 3) void attn_dkv_ke
   constexpr int TB = Dkv<DP>::TB, DKV_ROWS = Dkv<DP>::ROWS, DKV_KEYS = Dkv<DP>::KEYS;
   extern __shared__ __attribute__((aligned(1024))) char dyn[];               // [buffer][Q, dO], V, [buffer][lse2, delta], tokens of the rows
   const int lane = threadIdx.x & 63, wave = (threadIdx.x >> 6) % Dkv<DP>::KW, rw = (threadIdx.x >> 6) / Dkv<DP>::KW;       // 32 keys, 32 rows of a tile
+  if (blockIdx.x >= p.blocks) {
+    clear_rows<DKV_WAVES * 64>(p.dk, p.clear_k, p.k_rows, p.kv_heads, p.dim, blockIdx.x - p.blocks, gridDim.x - p.blocks);
+    clear_rows<DKV_WAVES * 64>(p.dv, p.clear_k, p.k_rows, p.kv_heads, p.dim, blockIdx.x - p.blocks, gridDim.x - p.blocks);
+    return;
+  }
   const Item it = p.items[blockIdx.x / p.kv_heads];
   const int hk = blockIdx.x % p.kv_heads;
   if (!item_ok(it, p) || it.first >= it.k_len || it.slot >= p.n_slots) return;
@@ -827,18 +853,20 @@ bool view_ok(const View& t, long tokens, long heads, int dim) {
          64 * t.st + 32 * t.sh + dim * 2 < (1l << 31);
 }
 
-template <typename T, int DP, int NW> int launch_fwd(const Params& p, long blocks, hipStream_t st) {
-  hipLaunchKernelGGL((attn_fwd_kernel<T, DP, NW>), dim3((unsigned)blocks), dim3(NW * 64), 0, st, p);
+unsigned clear_blocks(long rows, long heads, int dim) { return (unsigned)std::min<long>(1024, (rows * heads * dim * 2 + CLEAR_BYTES - 1) / CLEAR_BYTES); }
+
+template <typename T, int DP, int NW> int launch_fwd(const Params& p, unsigned more, hipStream_t st) {
+  if (p.blocks + more == 0) return DH_OK;
+  hipLaunchKernelGGL((attn_fwd_kernel<T, DP, NW>), dim3(p.blocks + more), dim3(NW * 64), 0, st, p);
   DH_LAUNCH_CHECK();
   return DH_OK;
 }
 template <typename T, int DP> int run_fwd(Params p, const dh_attn_info& info, const Item* items, hipStream_t st) {
   p.items = items;
-  const long blocks = info.n_fwd * info.kv_heads;
-  if (blocks) {
-    const int rc = info.waves == 1 ? launch_fwd<T, DP, 1>(p, blocks, st) : info.waves == 4 ? launch_fwd<T, DP, 4>(p, blocks, st) : launch_fwd<T, DP, 8>(p, blocks, st);
-    if (rc != DH_OK) return rc;
-  }
+  p.blocks = (int)(info.n_fwd * info.kv_heads);
+  const unsigned more = clear_blocks(p.q_rows - p.clear_q, p.heads, p.dim);
+  const int rc = info.waves == 1 ? launch_fwd<T, DP, 1>(p, more, st) : launch_fwd<T, DP, 4>(p, more, st);
+  if (rc != DH_OK) return rc;
   if (info.n_join) {
     p.items = items + info.n_fwd;
     const int rows = (int)info.waves * 32;
@@ -849,14 +877,18 @@ template <typename T, int DP> int run_fwd(Params p, const dh_attn_info& info, co
 }
 template <typename T, int DP> int run_bwd(Params p, const dh_attn_info& info, const Item* items, hipStream_t st) {
   p.items = items + info.n_fwd + info.n_join;
-  if (info.n_dq) {
-    hipLaunchKernelGGL((attn_dq_kernel<T, DP, 4>), dim3((unsigned)(info.n_dq * info.kv_heads)), dim3(256), 0, st, p);
+  p.blocks = (int)(info.n_dq * info.kv_heads);
+  unsigned more = clear_blocks(p.q_rows - p.clear_q, p.heads, p.dim);
+  if (p.blocks + more) {
+    hipLaunchKernelGGL((attn_dq_kernel<T, DP, 4>), dim3(p.blocks + more), dim3(256), 0, st, p);
     DH_LAUNCH_CHECK();
   }
   p.items += info.n_dq;
-  if (info.n_dkv) {
+  p.blocks = (int)(info.n_dkv * info.kv_heads);
+  more = clear_blocks(p.k_rows - p.clear_k, p.kv_heads, p.dim);
+  if (p.blocks + more) {
     DH_LDS_OPTIN((attn_dkv_kernel<T, DP>), Dkv<DP>::LDS);
-    hipLaunchKernelGGL((attn_dkv_kernel<T, DP>), dim3((unsigned)(info.n_dkv * info.kv_heads)), dim3(DKV_WAVES * 64), Dkv<DP>::LDS, st, p);
+    hipLaunchKernelGGL((attn_dkv_kernel<T, DP>), dim3(p.blocks + more), dim3(DKV_WAVES * 64), Dkv<DP>::LDS, st, p);
     DH_LAUNCH_CHECK();
   }
   p.items += info.n_dkv;
@@ -868,9 +900,9 @@ template <typename T, int DP> int run_bwd(Params p, const dh_attn_info& info, co
 }
 
 bool info_ok(const dh_attn_info* i) {
-  return i && heads_ok(i->heads, i->kv_heads, i->head_dim) && i->causal_block >= 0 && i->causal_block <= MAX_ROWS && (i->waves == 1 || i->waves == 4 || i->waves == 8) &&
+  return i && heads_ok(i->heads, i->kv_heads, i->head_dim) && i->causal_block >= 0 && i->causal_block <= MAX_ROWS && (i->waves == 1 || i->waves == 4) &&
          i->n_fwd >= 0 && i->n_join >= 0 && i->n_dq >= 0 && i->n_dkv >= 0 && i->n_dkv_join >= 0 && i->n_slots >= 0 && i->n_dkv_slots >= 0 && i->q_rows >= 0 && i->k_rows >= 0 && i->q_rows <= MAX_ROWS && i->k_rows <= MAX_ROWS &&
-         i->n_fwd * i->kv_heads <= INT_MAX && i->n_join * i->kv_heads <= 65535 && i->n_dq * i->kv_heads <= INT_MAX && i->n_dkv * i->kv_heads <= INT_MAX && i->n_dkv_join * i->kv_heads <= 65535;
+         i->n_fwd * i->kv_heads <= INT_MAX - 1024 && i->n_join * i->kv_heads <= 65535 && i->n_dq * i->kv_heads <= INT_MAX - 1024 && i->n_dkv * i->kv_heads <= INT_MAX - 1024 && i->n_dkv_join * i->kv_heads <= 65535;
 }
 
 }  // namespace
@@ -1019,20 +1051,20 @@ extern "C" size_t dh_attn_fwd_workspace_bytes(const dh_attn_info* info) {
 
 extern "C" int dh_attn_fwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh,
                            void* o, int64_t o_st, int64_t o_sh, void* o_low, float* lse, const int32_t* plan, const dh_attn_info* info, int dtype, int64_t q_rows,
-                           int64_t k_rows, float scale, void* workspace, size_t workspace_bytes, dh_stream_t stream) {
+                           int64_t k_rows, float scale, int clear_rest, void* workspace, size_t workspace_bytes, dh_stream_t stream) {
   if (!info_ok(info) || (dtype != DH_F16 && dtype != DH_BF16) || q_rows < info->q_rows || k_rows < info->k_rows || q_rows > MAX_ROWS || k_rows > MAX_ROWS ||
       !(scale > 0.f) || !(scale < 1e30f)) return DH_ERR_ARG;
-  if (info->n_fwd == 0) return DH_OK;
+  if (info->n_fwd == 0 && !(clear_rest && q_rows)) return DH_OK;
   Params p;
   memset(&p, 0, sizeof p);
   p.q = {(const char*)q, q_st * 2, q_sh * 2}; p.k = {(const char*)k, k_st * 2, k_sh * 2}; p.v = {(const char*)v, v_st * 2, v_sh * 2}; p.o = {(const char*)o, o_st * 2, o_sh * 2};
   const int dim = (int)info->head_dim;
-  if (!plan || !lse || ((unsigned long)o_low & 15) || !view_ok(p.q, q_rows, info->heads, dim) || !view_ok(p.o, q_rows, info->heads, dim)) return DH_ERR_ARG;
+  if ((info->ints && !plan) || !lse || ((unsigned long)o_low & 15) || !view_ok(p.q, q_rows, info->heads, dim) || !view_ok(p.o, q_rows, info->heads, dim)) return DH_ERR_ARG;
   if (info->k_rows && (!view_ok(p.k, k_rows, info->kv_heads, dim) || !view_ok(p.v, k_rows, info->kv_heads, dim))) return DH_ERR_ARG;
   if (info->n_slots && (!workspace || ((unsigned long)workspace & 15) || workspace_bytes < dh_attn_fwd_workspace_bytes(info))) return DH_ERR_WORKSPACE;
   p.low = (char*)o_low; p.lse = lse; p.part = (float*)workspace; p.n_slots = info->n_slots;
   p.kv_heads = (int)info->kv_heads; p.heads = (int)info->heads; p.group = p.heads / p.kv_heads; p.dim = dim; p.block = (int)info->causal_block;
-  p.q_rows = (int)q_rows; p.k_rows = (int)k_rows; p.scale = scale; p.c = scale * LOG2E;
+  p.q_rows = (int)q_rows; p.k_rows = (int)k_rows; p.clear_q = clear_rest ? (int)info->q_rows : p.q_rows; p.clear_k = clear_rest ? (int)info->k_rows : p.k_rows; p.scale = scale; p.c = scale * LOG2E;
   const Item* items = reinterpret_cast<const Item*>(plan);
   hipStream_t st = (hipStream_t)stream;
   const int dp = pad_dim(dim);
@@ -1049,27 +1081,30 @@ extern "C" size_t dh_attn_bwd_workspace_bytes(const dh_attn_info* info) {
 extern "C" int dh_attn_bwd(const void* grad, int64_t g_st, int64_t g_sh, const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh,
                            const void* v, int64_t v_st, int64_t v_sh, const void* o, int64_t o_st, int64_t o_sh, const void* o_low, const float* lse, void* dq, int64_t dq_st,
                            int64_t dq_sh, void* dk, int64_t dk_st, int64_t dk_sh, void* dv, int64_t dv_st, int64_t dv_sh, const int32_t* plan,
-                           const dh_attn_info* info, int dtype, int64_t q_rows, int64_t k_rows, float scale, void* workspace, size_t workspace_bytes,
-                           dh_stream_t stream) {
+                           const dh_attn_info* info, int dtype, int64_t q_rows, int64_t k_rows, float scale, int clear_rest, void* workspace,
+                           size_t workspace_bytes, dh_stream_t stream) {
   if (!info_ok(info) || info->keys_shared || (dtype != DH_F16 && dtype != DH_BF16) || q_rows < info->q_rows || k_rows < info->k_rows || q_rows > MAX_ROWS ||
       k_rows > MAX_ROWS || !(scale > 0.f) || !(scale < 1e30f)) return DH_ERR_ARG;
-  if (info->n_dq == 0 && info->n_dkv == 0) return DH_OK;
+  const bool rest_q = clear_rest && q_rows > info->q_rows, rest_k = clear_rest && k_rows > info->k_rows;
+  if (info->n_dq == 0 && info->n_dkv == 0 && !rest_q && !rest_k) return DH_OK;
   Params p;
   memset(&p, 0, sizeof p);
   p.q = {(const char*)q, q_st * 2, q_sh * 2}; p.k = {(const char*)k, k_st * 2, k_sh * 2}; p.v = {(const char*)v, v_st * 2, v_sh * 2}; p.o = {(const char*)o, o_st * 2, o_sh * 2};
   p.g = {(const char*)grad, g_st * 2, g_sh * 2}; p.dq = {(const char*)dq, dq_st * 2, dq_sh * 2}; p.dk = {(const char*)dk, dk_st * 2, dk_sh * 2}; p.dv = {(const char*)dv, dv_st * 2, dv_sh * 2};
   const int dim = (int)info->head_dim;
-  if (!plan) return DH_ERR_ARG;
+  if (info->ints && !plan) return DH_ERR_ARG;
   if (info->n_dq) {
     if (!lse || ((unsigned long)o_low & 15) || !view_ok(p.q, q_rows, info->heads, dim) || !view_ok(p.o, q_rows, info->heads, dim) || !view_ok(p.g, q_rows, info->heads, dim) ||
         !view_ok(p.dq, q_rows, info->heads, dim)) return DH_ERR_ARG;
     if (!workspace || ((unsigned long)workspace & 15) || workspace_bytes < dh_attn_bwd_workspace_bytes(info)) return DH_ERR_WORKSPACE;
   }
+  if (rest_q && !view_ok(p.dq, q_rows, info->heads, dim)) return DH_ERR_ARG;
+  if (rest_k && (!view_ok(p.dk, k_rows, info->kv_heads, dim) || !view_ok(p.dv, k_rows, info->kv_heads, dim))) return DH_ERR_ARG;
   if (info->n_dkv && (!view_ok(p.k, k_rows, info->kv_heads, dim) || !view_ok(p.v, k_rows, info->kv_heads, dim) || !view_ok(p.dk, k_rows, info->kv_heads, dim) ||
                       !view_ok(p.dv, k_rows, info->kv_heads, dim))) return DH_ERR_ARG;
   p.low = (char*)const_cast<void*>(o_low); p.lse = const_cast<float*>(lse); p.delta = (float*)workspace; p.part = (float*)workspace + delta_floats(info); p.n_slots = info->n_dkv_slots;
   p.kv_heads = (int)info->kv_heads; p.heads = (int)info->heads; p.group = p.heads / p.kv_heads; p.dim = dim; p.block = (int)info->causal_block;
-  p.q_rows = (int)q_rows; p.k_rows = (int)k_rows; p.scale = scale; p.c = scale * LOG2E;
+  p.q_rows = (int)q_rows; p.k_rows = (int)k_rows; p.clear_q = clear_rest ? (int)info->q_rows : p.q_rows; p.clear_k = clear_rest ? (int)info->k_rows : p.k_rows; p.scale = scale; p.c = scale * LOG2E;
   const Item* items = reinterpret_cast<const Item*>(plan);
   hipStream_t st = (hipStream_t)stream;
   const int dp = pad_dim(dim);

@@ -874,11 +874,8 @@ std::vector<torch::Tensor> attention_forward(torch::Tensor q, torch::Tensor k, t
   const size_t wsb = dh_attn_fwd_workspace_bytes(&i);
   torch::Tensor ws = torch::empty({(int64_t)wsb}, q.options().dtype(torch::kUInt8));
   check_status(dh_attn_fwd(TOKEN_VIEW(q), TOKEN_VIEW(k), TOKEN_VIEW(v), TOKEN_VIEW(o), for_backward ? low.data_ptr() : nullptr, lse.data_ptr<float>(),
-                           plan.data_ptr<int32_t>(), &i, dt, q.size(0), k.size(0), (float)scale, ws.data_ptr(), wsb, stream_of(q)), "attention_forward");
-  if (q.size(0) > i.q_rows) {
-    if (!out) o.narrow(0, i.q_rows, q.size(0) - i.q_rows).zero_();
-    lse.narrow(0, i.q_rows, q.size(0) - i.q_rows).fill_(-std::numeric_limits<float>::infinity());
-  }
+                           plan.data_ptr<int32_t>(), &i, dt, q.size(0), k.size(0), (float)scale, !out, ws.data_ptr(), wsb, stream_of(q)), "attention_forward");
+  if (out && q.size(0) > i.q_rows) lse.narrow(0, i.q_rows, q.size(0) - i.q_rows).fill_(-std::numeric_limits<float>::infinity());
   return {o, lse, low};
 }
 
@@ -905,13 +902,29 @@ std::vector<torch::Tensor> attention_backward(torch::Tensor grad, torch::Tensor 
   const size_t wsb = dh_attn_bwd_workspace_bytes(&i);
   torch::Tensor ws = torch::empty({(int64_t)wsb}, q.options().dtype(torch::kUInt8));
   check_status(dh_attn_bwd(TOKEN_VIEW(grad), TOKEN_VIEW(q), TOKEN_VIEW(k), TOKEN_VIEW(v), TOKEN_VIEW(o), low ? low->data_ptr() : nullptr, lse.data_ptr<float>(), TOKEN_VIEW(dq), TOKEN_VIEW(dk), TOKEN_VIEW(dv),
-                           plan.data_ptr<int32_t>(), &i, dt, q.size(0), k.size(0), (float)scale, ws.data_ptr(), wsb, stream_of(q)), "attention_backward");
-  if (q.size(0) > i.q_rows) dq.narrow(0, i.q_rows, q.size(0) - i.q_rows).zero_();
-  if (!gaps && k.size(0) > i.k_rows) {
-    dk.narrow(0, i.k_rows, k.size(0) - i.k_rows).zero_();
-    dv.narrow(0, i.k_rows, k.size(0) - i.k_rows).zero_();
-  }
+                           plan.data_ptr<int32_t>(), &i, dt, q.size(0), k.size(0), (float)scale, 1, ws.data_ptr(), wsb, stream_of(q)), "attention_backward");
   return {dq, dk, dv};
+}
+
+// the same with a gradient (once): what droid_amd.attention.packed_attention calls where one is wanted
+struct PackedAttention : public torch::autograd::Function<PackedAttention> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor plan, torch::Tensor info,
+                                                double scale) {
+    auto r = attention_forward(q, k, v, plan, info, scale, c10::nullopt, true);
+    ctx->save_for_backward({q, k, v, r[0], r[1], r[2], plan, info});
+    ctx->saved_data["scale"] = scale;
+    ctx->mark_non_differentiable({r[1]});
+    return {r[0], r[1]};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), "packed_attention is differentiable once (create_graph is not supported)");
+    const auto s = ctx->get_saved_variables();
+    auto r = attention_backward(grads[0], s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], ctx->saved_data["scale"].toDouble());
+    return {r[0], r[1], r[2], torch::Tensor(), torch::Tensor(), torch::Tensor()};
+  }
+};
+std::vector<torch::Tensor> packed_attention(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor plan, torch::Tensor info, double scale) {
+  return PackedAttention::apply(q, k, v, plan, info, scale);
 }
 
 struct RopeArgs { std::vector<int> sections; int pos_type, w_dtype; const void *qw, *kw; };
@@ -998,6 +1011,35 @@ std::vector<torch::Tensor> qk_norm_rope_backward(torch::Tensor dq_out, torch::Te
   return {dq, dk, dqw, dkw};
 }
 
+struct QkNormRope : public torch::autograd::Function<QkNormRope> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, torch::Tensor q, torch::Tensor k, torch::Tensor positions, torch::Tensor inv_freq,
+                                                c10::optional<torch::Tensor> q_weight, c10::optional<torch::Tensor> k_weight, std::vector<int64_t> sections, bool normalize,
+                                                double eps, bool interleaved) {
+    auto r = qk_norm_rope_forward(q, k, positions, inv_freq, sections, q_weight, k_weight, normalize, eps, interleaved, c10::nullopt, c10::nullopt);
+    // (a rotation alone needs no input for its gradient)
+    ctx->save_for_backward({normalize ? q : torch::Tensor(), normalize ? k : torch::Tensor(), positions, inv_freq, q_weight.value_or(torch::Tensor()), k_weight.value_or(torch::Tensor())});
+    ctx->saved_data["sections"] = sections;
+    ctx->saved_data["normalize"] = normalize;
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["interleaved"] = interleaved;
+    return {r[0], r[1]};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), "qk_norm_rope is differentiable once (create_graph is not supported)");
+    const auto s = ctx->get_saved_variables();
+    const bool normalize = ctx->saved_data["normalize"].toBool();
+    const auto opt = [](const torch::Tensor& t) { return t.defined() ? c10::optional<torch::Tensor>(t) : c10::nullopt; };
+    auto r = qk_norm_rope_backward(grads[0], grads[1], normalize ? s[0] : grads[0], normalize ? s[1] : grads[1], s[2], s[3], ctx->saved_data["sections"].toIntVector(), opt(s[4]),
+                                   opt(s[5]), normalize, ctx->saved_data["eps"].toDouble(), ctx->saved_data["interleaved"].toBool());
+    const torch::Tensor none;
+    return {r[0], r[1], none, none, s[4].defined() ? r[2] : none, s[5].defined() ? r[3] : none, none, none, none, none};
+  }
+};
+std::vector<torch::Tensor> qk_norm_rope(torch::Tensor q, torch::Tensor k, torch::Tensor positions, torch::Tensor inv_freq, const std::vector<int64_t>& sections,
+                                        c10::optional<torch::Tensor> q_weight, c10::optional<torch::Tensor> k_weight, bool normalize, double eps, bool interleaved) {
+  return QkNormRope::apply(q, k, positions, inv_freq, q_weight, k_weight, sections, normalize, eps, interleaved);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -1071,6 +1113,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("attention_forward", &attention_forward, "packed softmax attention: {o, lse, o_low}", py::arg("q"), py::arg("k"), py::arg("v"), py::arg("plan"), py::arg("info"),
         py::arg("scale"), py::arg("out") = py::none(), py::arg("for_backward") = false);
   m.def("attention_backward", &attention_backward, "gradients of packed softmax attention: {dq, dk, dv}");
+  m.def("packed_attention", &packed_attention, "attention_forward with a gradient: {o, lse}");
+  m.def("qk_norm_rope", &qk_norm_rope, "qk_norm_rope_forward with a gradient: {q, k}");
   m.def("qk_norm_rope_forward", &qk_norm_rope_forward, "norm of query / key heads and rotation by position: {q, k}", py::arg("q"), py::arg("k"), py::arg("positions"),
         py::arg("inv_freq"), py::arg("sections"), py::arg("q_weight") = py::none(), py::arg("k_weight") = py::none(), py::arg("normalize") = true, py::arg("eps") = 1e-6,
         py::arg("interleaved") = false, py::arg("q_out") = py::none(), py::arg("k_out") = py::none());

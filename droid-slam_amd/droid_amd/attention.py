@@ -14,7 +14,6 @@ PackedPlan (a copy to the device: build it before a graph is captured)."""
 import math
 
 import torch
-from torch.autograd.function import once_differentiable
 
 import droid_backends
 
@@ -42,23 +41,6 @@ class PackedPlan:
         self.device = self.items.device
 
 
-class _PackedAttention(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, plan, scale):
-        o, lse, low = droid_backends.attention_forward(q, k, v, plan.items, plan.info, scale, None, True)
-        ctx.save_for_backward(q, k, v, o, lse, low)
-        ctx.plan, ctx.scale = plan, scale
-        ctx.mark_non_differentiable(lse)
-        return o, lse
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad, _):
-        q, k, v, o, lse, low = ctx.saved_tensors
-        dq, dk, dv = droid_backends.attention_backward(grad, q, k, v, o, lse, low, ctx.plan.items, ctx.plan.info, ctx.scale)
-        return dq, dk, dv, None, None
-
-
 def packed_attention(q, k, v, plan, scale=None, out=None, return_lse=False):
     """softmax(scale q k^T) v for every sequence of `plan`: q [rows, heads, head_dim], k and v [key rows, kv_heads, head_dim], float16 or
     bfloat16, any strides between rows and heads.  scale > 0 (default 1 / sqrt(head_dim)).  Query head n reads key head
@@ -71,28 +53,10 @@ def packed_attention(q, k, v, plan, scale=None, out=None, return_lse=False):
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         if out is not None:
             raise RuntimeError("packed_attention: out= takes no gradient; leave it out or use torch.no_grad()")
-        o, lse = _PackedAttention.apply(q, k, v, plan, scale)
+        o, lse = droid_backends.packed_attention(q, k, v, plan.items, plan.info, scale)
     else:
         o, lse, _ = droid_backends.attention_forward(q, k, v, plan.items, plan.info, scale, out)
     return (o, lse) if return_lse else o
-
-
-class _QkNormRope(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, positions, inv_freq, q_weight, k_weight, sections, normalize, eps, interleaved):
-        qo, ko = droid_backends.qk_norm_rope_forward(q, k, positions, inv_freq, sections, q_weight, k_weight, normalize, eps, interleaved)
-        ctx.rule = (sections, normalize, eps, interleaved)
-        ctx.save_for_backward(*((q, k) if normalize else ()), positions, inv_freq, q_weight, k_weight)
-        return qo, ko
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dqo, dko):
-        sections, normalize, eps, interleaved = ctx.rule
-        *x, positions, inv_freq, q_weight, k_weight = ctx.saved_tensors
-        q, k = x if normalize else (dqo, dko)                   # a rotation alone needs no input for its gradient
-        dq, dk, dqw, dkw = droid_backends.qk_norm_rope_backward(dqo, dko, q, k, positions, inv_freq, sections, q_weight, k_weight, normalize, eps, interleaved)
-        return dq, dk, None, None, None if q_weight is None else dqw, None if k_weight is None else dkw, None, None, None, None
 
 
 def qk_norm_rope(q, k, positions, inv_freq, sections, q_weight=None, k_weight=None, *, normalize=True, eps=1e-6, interleaved=False, out=None):
@@ -109,6 +73,6 @@ def qk_norm_rope(q, k, positions, inv_freq, sections, q_weight=None, k_weight=No
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
         if out is not None:
             raise RuntimeError("qk_norm_rope: out= takes no gradient; leave it out or use torch.no_grad()")
-        return _QkNormRope.apply(q, k, positions, inv_freq, q_weight, k_weight, sections, bool(normalize), float(eps), bool(interleaved))
+        return tuple(droid_backends.qk_norm_rope(q, k, positions, inv_freq, sections, q_weight, k_weight, bool(normalize), float(eps), bool(interleaved)))
     qo, ko = out if out is not None else (None, None)
     return tuple(droid_backends.qk_norm_rope_forward(q, k, positions, inv_freq, sections, q_weight, k_weight, bool(normalize), float(eps), bool(interleaved), qo, ko))

@@ -481,7 +481,8 @@ int dh_reproject_ex(const float* poses, const float* disps, const float* intrins
  * min(k_len, (floor((i + k_len - q_len) / causal_block) + 1) * causal_block): 1 = token by token, the last token standing at the last key;
  * n = whole blocks (keyframes) of n keys.  A row that sees nothing: o = 0, lse = -inf, gradients 0.
  *   o = softmax(scale q k^T) v (scale > 0), lse [q_rows, heads] f32 = natural logarithm of the row's sum.
- * Rows of o, lse, dq behind the last sequence, and rows of dk, dv that belong to no sequence, are left as they were.
+ * Rows behind the last sequence (of o, lse, dq) and behind the last key (of dk, dv) are left as they were, or cleared where clear_rest
+ * (o, gradients 0, lse -inf).  Rows of dk, dv between the sequences' keys (k_start with gaps) are left as they were.
  * Values are expected to be finite where a gradient is wanted.  A non-finite value (q, k or v) reaches the rows that see it and no others.
  *
  * dh_attn_plan runs on the HOST: it lays out the work items of one set of lengths.  plan_host NULL: only fills *info (info->ints = ints
@@ -508,13 +509,13 @@ size_t dh_attn_bwd_workspace_bytes(const dh_attn_info* info_host);
 int dh_attn_fwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh,
                 const void* v, int64_t v_st, int64_t v_sh, void* o, int64_t o_st, int64_t o_sh, void* o_low, float* lse,
                 const int32_t* plan, const dh_attn_info* info_host, int dtype, int64_t q_rows, int64_t k_rows, float scale,
-                void* workspace, size_t workspace_bytes, dh_stream_t stream);
+                int clear_rest, void* workspace, size_t workspace_bytes, dh_stream_t stream);
 int dh_attn_bwd(const void* grad, int64_t g_st, int64_t g_sh, const void* q, int64_t q_st, int64_t q_sh,
                 const void* k, int64_t k_st, int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh,
                 const void* o, int64_t o_st, int64_t o_sh, const void* o_low, const float* lse,
                 void* dq, int64_t dq_st, int64_t dq_sh, void* dk, int64_t dk_st, int64_t dk_sh, void* dv, int64_t dv_st, int64_t dv_sh,
                 const int32_t* plan, const dh_attn_info* info_host, int dtype, int64_t q_rows, int64_t k_rows, float scale,
-                void* workspace, size_t workspace_bytes, dh_stream_t stream);
+                int clear_rest, void* workspace, size_t workspace_bytes, dh_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------------
  * Norm of every query and key head and rotation by the token's position, in one pass, forward and backward.

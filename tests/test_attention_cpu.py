@@ -111,7 +111,7 @@ def test_c_entries_refuse_before_a_launch():
 
     def fwd(q=256, k=256, v=256, o=256, low=0, lse=256, plan=256, dtype=0, rows=5, keys=9, scale=0.1, st=(256, 64), ws=0, wsb=0, info=info):
         t = lambda p: (ptr(p), i64(st[0]), i64(st[1]))  # noqa: E731
-        return lib.dh_attn_fwd(*t(q), *t(k), *t(v), *t(o), ptr(low), ptr(lse), ptr(plan), info, dtype, i64(rows), i64(keys), ctypes.c_float(scale), ptr(ws), ctypes.c_size_t(wsb), ptr(0))
+        return lib.dh_attn_fwd(*t(q), *t(k), *t(v), *t(o), ptr(low), ptr(lse), ptr(plan), info, dtype, i64(rows), i64(keys), ctypes.c_float(scale), 0, ptr(ws), ctypes.c_size_t(wsb), ptr(0))
 
     make([5], [9])
     for bad in (dict(q=0), dict(q=8), dict(k=0), dict(v=264), dict(o=0), dict(low=8), dict(lse=0), dict(plan=0), dict(dtype=1), dict(dtype=2), dict(rows=4), dict(keys=8), dict(scale=0.0),
@@ -122,7 +122,7 @@ def test_c_entries_refuse_before_a_launch():
 
     def bwd(ws=256, wsb=1 << 20, dtype=0, rows=5, keys=9, dq=256, dk=256, plan=256, lse=256):
         t = lambda p: (ptr(p), i64(256), i64(64))  # noqa: E731
-        return lib.dh_attn_bwd(*t(256), *t(256), *t(256), *t(256), *t(256), ptr(0), ptr(lse), *t(dq), *t(dk), *t(256), ptr(plan), info, dtype, i64(rows), i64(keys), ctypes.c_float(0.1),
+        return lib.dh_attn_bwd(*t(256), *t(256), *t(256), *t(256), *t(256), ptr(0), ptr(lse), *t(dq), *t(dk), *t(256), ptr(plan), info, dtype, i64(rows), i64(keys), ctypes.c_float(0.1), 0,
                                ptr(ws), ctypes.c_size_t(wsb), ptr(0))
 
     make([5], [9])
