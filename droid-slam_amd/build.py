@@ -195,6 +195,23 @@ def audit_spills(force=False, verbose=False):
     open(stamp, "w").write("%d instantiations, no scratch\n" % seen)
 
 
+def audit_m0(force=False, verbose=False):
+    """attention.hip sets m0 for its LDS-DMA in inline asm and does not restore it: require that nothing else in the generated ISA names m0."""
+    import re
+    src = os.path.join(CSRC, "attention.hip")
+    stamp = os.path.join(OBJ, "attention.m0_audit_ok")
+    if not force and os.path.exists(stamp) and os.path.getmtime(stamp) >= max(os.path.getmtime(src), *map(os.path.getmtime, headers())):
+        return
+    asm = os.path.join(OBJ, "attention.s")
+    _run([HIPCC] + HIP_FLAGS + ["-S", "--cuda-device-only", src, "-o", asm], verbose)
+    lines = open(asm).read().splitlines()
+    named = [i for i, l in enumerate(lines) if re.search(r"\bm0\b", l.split(";")[0])]
+    bad = [lines[i] for i in named if not (lines[i].split()[:2] == ["s_mov_b32", "m0,"] and lines[i + 2].split()[0] == "buffer_load_dwordx4" and lines[i + 2].endswith("lds"))]
+    if bad or not named:
+        raise RuntimeError("m0 outside the LDS-DMA of attention.hip:\n" + "\n".join(bad[:10] or ["no LDS-DMA found"]))
+    open(stamp, "w").write("%d LDS-DMA instructions\n" % len(named))
+
+
 def build_ext(force=False, verbose=False):
     import torch
     from torch.utils import cpp_extension as ce
@@ -224,6 +241,7 @@ def build_all(force=False, verbose=False):
     if not SANITIZE:                      # (the ISA audits judge the release flags)
         audit_asm_loads(force, verbose)
         audit_spills(force, verbose)
+        audit_m0(force, verbose)
     build_ext(force, verbose)
     return LIB, EXT
 

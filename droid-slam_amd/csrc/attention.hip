@@ -15,8 +15,8 @@
 //
 // Memory.  64-row tiles arrive by LDS-DMA (buffer_load_dwordx4 ... lds) in two buffers, the next tile under the current one's products;
 // rows behind the end and channels behind head_dim are out of the buffer's range and arrive as zeros.  The 16-byte chunks of a row are
-// stored at chunk ^ swz(row): eight consecutive rows at one chunk (the K operand) and four consecutive rows at two (a transposed read)
-// fall on different banks.
+// stored at chunk ^ swz(row): sixteen consecutive rows at one chunk (the K operand) and four consecutive rows at four (half a wave's transposed
+// read) fall on different banks.
 //
 // Precision.  Products of 16-bit operands accumulate in 32 bits; scores, statistics, p, dP, delta and all accumulators are 32-bit.
 // p and dS are rounded (to nearest) to the inputs' type as operands of the second product: their relative error is the same half step
@@ -103,8 +103,8 @@ template <int DP> struct Geo {
   static constexpr int ROWB = DP * 2, CH = DP / 8, TILEB = BN * ROWB;
   static __device__ __forceinline__ int swz(int r) {
     const int low = (r >> 3) & 1;
-    if constexpr (DP == 128) return ((r & 7) << 1) | low;
-    else if constexpr (DP == 64) return (((r >> 1) & 3) << 1) | low;
+    if constexpr (DP == 128) return ((r & 3) << 2) | (((r >> 2) & 1) << 1) | low;
+    else if constexpr (DP == 64) return (((r >> 1) & 1) << 2) | (((r >> 2) & 1) << 1) | low;
     else return (((r >> 2) & 1) << 1) | low;
   }
 };
@@ -114,22 +114,21 @@ __device__ __forceinline__ long uniform(long x) {
                 (unsigned)__builtin_amdgcn_readfirstlane((int)x));
 }
 
-// the buffer of everything from `p` on (raw, 2^31 - 1 bytes)
-__device__ __forceinline__ i32x4 buffer_at(const char* p) {
+// the buffer of `bytes` bytes from `p` on (raw); both uniform
+__device__ __forceinline__ i32x4 buffer_at(const char* p, unsigned bytes) {
   const unsigned long a = (unsigned long)p;
   i32x4 s;
   s.x = __builtin_amdgcn_readfirstlane((int)a);
   s.y = __builtin_amdgcn_readfirstlane((int)(a >> 32) & 0xffff);
-  s.z = 0x7fffffff;
+  s.z = __builtin_amdgcn_readfirstlane((int)bytes);
   s.w = 0x00027000;
   return s;
 }
 
-// lane l copies 16 bytes at buffer + voff (per lane) to LDS address lds + 16 l; zeros where voff is out of range
+// lane l copies 16 bytes at buffer + voff (per lane) to LDS address lds + 16 l; zeros where voff is out of range.  m0 is not kept: the compiler
+// has no use for it in these kernels (build.py looks at the generated code), and saving it costs two more instructions a chunk.
 __device__ __forceinline__ void dma16(i32x4 buffer, unsigned voff, unsigned lds) {
-  unsigned keep;
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds\n\ts_mov_b32 m0, %0"
-               : "=&s"(keep) : "v"(voff), "s"(buffer), "s"(lds) : "memory");
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" : : "v"(voff), "s"(buffer), "s"(lds) : "memory");
 }
 // keeps a branch a branch: without it the selects of masked tiles are executed (and waited for) in every tile
 #define RARE_BRANCH() asm volatile("")
@@ -140,12 +139,13 @@ template <int LEFT, bool BARRIER> __device__ __forceinline__ void dma_wait() {
 }
 #define DMA_WAIT_BARRIER() asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory")
 
-// One tensor's 64-row tiles through LDS-DMA by NW waves.  Tile row x is token x / group (from the tile's first token on) and head x % group;
-// a key tensor has group 1.
-template <int DP, int NW, int ROWS = BN> struct TileLoader {
+// One tensor's tiles of ROWS rows through LDS-DMA by NW waves.  Tile row x is token x / group (from the tile's first token on) and head
+// x % group.  Rows that do not exist are behind the buffer's end (BY_END: keys, one row a token, rows at least as far apart as they are long:
+// the host sees to it), or get an offset that is (heads may be further apart than tokens).
+template <int DP, int NW, int ROWS, bool BY_END> struct TileLoader {
   using G = Geo<DP>;
-  static constexpr int PER = (ROWS * G::CH + NW * 64 - 1) / (NW * 64);   // 16-byte chunks a thread
-  static constexpr int STEP = NW * 64 / G::CH;                         // rows between two of them
+  static constexpr int PER = (ROWS * G::CH + NW * 64 - 1) / (NW * 64);       // 16-byte chunks a thread
+  static constexpr int STEP = NW * 64 / G::CH;                               // rows between two of them
   unsigned voff[PER];
   __device__ __forceinline__ void init(const View& t, int dim, int group, int rows) {
 #pragma unroll
@@ -154,14 +154,14 @@ template <int DP, int NW, int ROWS = BN> struct TileLoader {
       voff[i] = r < rows && c * 8 < dim ? (unsigned)(tok * t.st + (r - tok * group) * t.sh + c * 16) : OUT_OF_RANGE;
     }
   }
-  // `rows`: tile rows that exist
-  __device__ __forceinline__ void issue(const char* tile, int rows, unsigned lds) const {
-    const i32x4 buffer = buffer_at(tile);
+  // `rows`: tile rows that exist (BY_END: `stride` bytes apart and `size` bytes long)
+  __device__ __forceinline__ void issue(const char* tile, int rows, unsigned stride, unsigned size, unsigned lds) const {
+    const i32x4 buffer = buffer_at(tile, !BY_END ? 0x7fffffffu : rows > 0 ? (unsigned)(min(rows, ROWS) - 1) * stride + size : 0u);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = threadIdx.x / G::CH;
     if (NW * 64 > ROWS * G::CH && wave * 64 >= ROWS * G::CH) return;
 #pragma unroll
     for (int i = 0; i < PER; ++i)
-      dma16(buffer, r + i * STEP < rows ? voff[i] : OUT_OF_RANGE, lds + (i * NW + wave) * 1024);
+      dma16(buffer, BY_END || r + i * STEP < rows ? voff[i] : OUT_OF_RANGE, lds + (i * NW + wave) * 1024);
   }
 };
 
@@ -304,7 +304,7 @@ __global__ __launch_bounds__(NW * 64, NW == 1 ? 1 : DP == 128 ? 2 : 3) void attn
   }
   f32x16 acc[DP / 32];
   float m, l;                                                                // l: this half's keys only
-  TileLoader<DP, NW, TK> lk, lv;
+  TileLoader<DP, NW, TK, true> lk, lv;
   lk.init(p.k, p.dim, 1, TK);
   lv.init(p.v, p.dim, 1, TK);
   const char* kp = p.k.p + uniform((long)(it.k_start + it.begin) * p.k.st + (long)hk * p.k.sh);
@@ -312,88 +312,128 @@ __global__ __launch_bounds__(NW * 64, NW == 1 ? 1 : DP == 128 ? 2 : 3) void attn
   lds_char* const lds = (lds_char*)smem;
   const unsigned lds0 = (unsigned)(unsigned long)lds;
   const int tiles = (key_end - it.begin + TK - 1) / TK;
-  auto issue = [&](int t) {
-    const unsigned to = lds0 + t % ST * 2 * TB;
-    const int left = key_end - it.begin - t * TK;                            // (behind the last tile: nothing, zeros go to a stage nobody reads)
-    lk.issue(kp + (long)t * TK * p.k.st, left, to);
-    lv.issue(vp + (long)t * TK * p.v.st, left, to + TB);
+  // the next K / V tile; behind the last one nothing is read, zeros go to a stage nobody reads
+  const unsigned k_st = (unsigned)p.k.st, v_st = (unsigned)p.v.st;
+  const char *k_next, *v_next;
+  int k_left, v_left, k_to, v_to;
+  auto issue_k = [&]() {
+    lk.issue(k_next, k_left, k_st, p.dim * 2, lds0 + k_to);
+    k_next += (long)TK * k_st;
+    k_left -= TK;
+    k_to = k_to == (ST - 1) * 2 * TB ? 0 : k_to + 2 * TB;
+  };
+  auto issue_v = [&]() {
+    lv.issue(v_next, v_left, v_st, p.dim * 2, lds0 + TB + v_to);
+    v_next += (long)TK * v_st;
+    v_left -= TK;
+    v_to = v_to == (ST - 1) * 2 * TB ? 0 : v_to + 2 * TB;
+  };
+  const auto k_tile = [&](int t) { return lds + t % ST * 2 * TB; };
+  const auto v_tile = [&](int t) { return lds + t % ST * 2 * TB + TB; };
+
+  // the scores of 32 keys: block b of a K tile
+  auto scores = [&](const lds_char* kt, int b) {
+    f32x16 s;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < DP / 16; ++ks) s = T::mfma(frag<DP>(kt, b, ks, lane), qf[ks], s);
+    return s;
+  };
+  // hides what a row does not see and keeps p at or below 2^8.  Each half of the wave looks at its own keys of a row; only where one of
+  // them found a maximum that is too large the halves agree on a new one.
+  auto settle = [&](f32x16& s, int n0) {
+    if (n0 + 32 > wmin) {
+      RARE_BRANCH();
+      const int end = lim - n0 - 4 * (lane >> 5);
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (8 * (i / 4) + (i & 3) >= end) s[i] = -INFINITY;
+    }
+    float mx = s[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
+    if (__any(mx * p.c > m + 8.f)) {
+      RARE_BRANCH();
+      mx = fmaxf(mx, other_half(mx)) * p.c;
+      const float mn = mx > m + 8.f ? mx : m, a = exp2_fast(m - mn);         // (a row's bits do not depend on its neighbours)
+      m = mn;
+      l *= a;
+#pragma unroll
+      for (int mb = 0; mb < DP / 32; ++mb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[mb][i] *= a;
+    }
+  };
+  auto soften = [&](f32x16& s, u32x4 (&pf)[2]) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      s[i] = exp2_fast(fmaf(s[i], p.c, -m));
+      l += s[i];
+    }
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) pf[ks][j] = T::pack(s[8 * ks + 2 * j], s[8 * ks + 2 * j + 1]);
   };
   auto walk = [&](auto careful) {
     constexpr bool CAREFUL = decltype(careful)::value;
     m = M_FLOOR;
     l = 0.f;
+    k_next = kp; v_next = vp;
+    k_left = v_left = key_end - it.begin;
+    k_to = v_to = 0;
 #pragma unroll
     for (int mb = 0; mb < DP / 32; ++mb)
 #pragma unroll
       for (int i = 0; i < 16; ++i) acc[mb][i] = 0.f;
-    for (int t = 0; t < ST - 1; ++t) issue(t);
-    for (int t = 0; t < tiles; ++t) {
-      // tile t is there (the stages behind it may still be on their way), and everybody has left tile t - 1
-      dma_wait<(ST - 2) * 2 * TileLoader<DP, NW, TK>::PER, (NW > 1)>();
-      issue(t + ST - 1);
-      const int n0 = it.begin + t * TK;
-      if (n0 >= wmax) continue;
-      const lds_char* kt = lds + t % ST * 2 * TB;
-      const lds_char* vt = kt + TB;
-      f32x16 s[KB];
+    auto add = [&](const lds_char* vt, int b, u32x4 (&pf)[2], int n0) {
 #pragma unroll
-      for (int b = 0; b < KB; ++b)
+      for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[b][i] = 0.f;
-#pragma unroll
-      for (int ks = 0; ks < DP / 16; ++ks)
-#pragma unroll
-        for (int b = 0; b < KB; ++b) s[b] = T::mfma(frag<DP>(kt, b, ks, lane), qf[ks], s[b]);
-      const bool masked = n0 + TK > wmin;
-      if (masked) {
-        RARE_BRANCH();
-        const int end = lim - n0 - 4 * (lane >> 5);
-#pragma unroll
-        for (int b = 0; b < KB; ++b)
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (b * 32 + 8 * (i / 4) + (i & 3) >= end) s[b][i] = -INFINITY;
-      }
-      float mx = s[0][0];
-#pragma unroll
-      for (int b = 0; b < KB; ++b)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[b][i]);
-      mx = fmaxf(mx, other_half(mx)) * p.c;
-      if (__any(mx > m + 8.f)) {
-        const float mn = mx > m + 8.f ? mx : m, a = exp2_fast(m - mn);       // (a row's bits do not depend on its neighbours)
-        m = mn;
-        l *= a;
-#pragma unroll
-        for (int mb = 0; mb < DP / 32; ++mb)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) acc[mb][i] *= a;
-      }
-      u32x4 pf[KB][2];
-#pragma unroll
-      for (int b = 0; b < KB; ++b) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          s[b][i] = exp2_fast(fmaf(s[b][i], p.c, -m));
-          l += s[b][i];
+        for (int mb = 0; mb < DP / 32; ++mb) {
+          const u32x4 vf = frag_t<DP>(vt, b, ks, mb, lane);
+          if (CAREFUL && n0 + 32 > wmin) add_seen<T>(acc[mb], vf, pf[ks], n0 + ks * 16 + 4 * (lane >> 5), lim);
+          else acc[mb] = T::mfma(vf, pf[ks], acc[mb]);
         }
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) pf[b][ks][j] = T::pack(s[b][8 * ks + 2 * j], s[b][8 * ks + 2 * j + 1]);
+    };
+    u32x4 pf[2];
+    if constexpr (NW == 1) {
+      for (int t = 0; t < ST - 1; ++t) { issue_k(); issue_v(); }
+      for (int t = 0; t < tiles; ++t) {
+        dma_wait<(ST - 2) * 2 * TileLoader<DP, NW, TK, true>::PER, false>();       // (the stages behind tile t may still be on their way)
+        issue_k();
+        issue_v();
+        const int n0 = it.begin + t * TK;
+        f32x16 s = scores(k_tile(t), 0);
+        settle(s, n0);
+        soften(s, pf);
+        add(v_tile(t), 0, pf, n0);
       }
-#pragma unroll
-      for (int b = 0; b < KB; ++b)
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-          for (int mb = 0; mb < DP / 32; ++mb) {
-            const u32x4 vf = frag_t<DP>(vt, b, ks, mb, lane);
-            if (CAREFUL && masked) add_seen<T>(acc[mb], vf, pf[b][ks], n0 + b * 32 + ks * 16 + 4 * (lane >> 5), lim);
-            else acc[mb] = T::mfma(vf, pf[b][ks], acc[mb]);
-          }
+    } else if (tiles > 0) {
+      // The next block's scores are formed (matrix cores) while the exponentials of this one are (vector units); so K runs ahead of V by a
+      // tile, and one barrier a tile serves both: before it K t and V t - 1 were read for the last time, behind it K t + 1 and V t are there.
+      issue_k();
+      dma_wait<0, true>();
+      issue_v();
+      issue_k();
+      f32x16 s = scores(k_tile(0), 0);
+      for (int t = 0; t < tiles; ++t) {
+        const int n0 = it.begin + t * TK;
+        settle(s, n0);
+        f32x16 s1 = scores(k_tile(t), 1);
+        soften(s, pf);
+        dma_wait<0, true>();
+        issue_v();
+        issue_k();
+        add(v_tile(t), 0, pf, n0);
+        settle(s1, n0 + 32);
+        s = scores(k_tile(t + 1), 0);                                        // (behind the last tile: zeros, not used)
+        soften(s1, pf);
+        add(v_tile(t), 1, pf, n0 + 32);
+      }
     }
-    dma_wait<0, false>();
+    dma_wait<0, (NW > 1)>();                                                 // (nothing may arrive later)
   };
   walk(std::false_type());
   // A value that is not finite makes 0 * v of the rows that do not see it NaN.  Only then the workgroup walks a second time.
@@ -548,7 +588,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_dq_kernel(const Params p) {
   for (int mb = 0; mb < DP / 32; ++mb)
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[mb][i] = 0.f;
-  TileLoader<DP, NW> lk, lv;
+  TileLoader<DP, NW, BN, true> lk, lv;
   lk.init(p.k, p.dim, 1, BN);
   lv.init(p.v, p.dim, 1, BN);
   const char* kp = p.k.p + uniform((long)(it.k_start + it.begin) * p.k.st + (long)hk * p.k.sh);
@@ -556,11 +596,15 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_dq_kernel(const Params p) {
   lds_char* const lds = (lds_char*)smem;
   const unsigned lds0 = (unsigned)(unsigned long)lds;
   const int tiles = (key_end - it.begin + BN - 1) / BN;
-  auto issue = [&](int t) {
+  int left = key_end - it.begin;
+  const unsigned k_st = (unsigned)p.k.st, v_st = (unsigned)p.v.st;
+  auto issue = [&](int t) {                                                  // in order
     const unsigned to = lds0 + (t & 1) * 2 * G::TILEB;
-    const int left = key_end - it.begin - t * BN;
-    lk.issue(kp + (long)t * BN * p.k.st, left, to);
-    lv.issue(vp + (long)t * BN * p.v.st, left, to + G::TILEB);
+    lk.issue(kp, left, k_st, p.dim * 2, to);
+    lv.issue(vp, left, v_st, p.dim * 2, to + G::TILEB);
+    kp += (long)BN * k_st;
+    vp += (long)BN * v_st;
+    left -= BN;
   };
   if (tiles > 0) issue(0);
   for (int t = 0; t < tiles; ++t) {
@@ -649,9 +693,9 @@ __global__ __launch_bounds__(DKV_WAVES * 64, DP == 128 ? 2 : 3) void attn_dkv_ke
   lds_char* const lds = (lds_char*)dyn;
   const unsigned lds0 = (unsigned)(unsigned long)lds;
   {
-    TileLoader<DP, DKV_WAVES, DKV_KEYS> l;
+    TileLoader<DP, DKV_WAVES, DKV_KEYS, true> l;
     l.init(p.v, p.dim, 1, DKV_KEYS);
-    l.issue(p.v.p + uniform((long)(it.k_start + it.first) * p.v.st + (long)hk * p.v.sh), it.k_len - it.first, lds0 + 4 * TB);
+    l.issue(p.v.p + uniform((long)(it.k_start + it.first) * p.v.st + (long)hk * p.v.sh), it.k_len - it.first, (unsigned)p.v.st, p.dim * 2, lds0 + 4 * TB);
   }
   u32x4 kf[DP / 16];
   {
@@ -669,7 +713,7 @@ __global__ __launch_bounds__(DKV_WAVES * 64, DP == 128 ? 2 : 3) void attn_dkv_ke
     for (int i = 0; i < 16; ++i) dk[mb][i] = dv[mb][i] = 0.f;
 
   const int tpt = DKV_ROWS / p.group;                                        // tokens a tile
-  TileLoader<DP, DKV_WAVES, DKV_ROWS> lq, lg;
+  TileLoader<DP, DKV_WAVES, DKV_ROWS, false> lq, lg;
   lq.init(p.q, p.dim, p.group, tpt * p.group);
   lg.init(p.g, p.dim, p.group, tpt * p.group);
   const int tok_end = min(it.end, it.q_len);
@@ -701,8 +745,10 @@ __global__ __launch_bounds__(DKV_WAVES * 64, DP == 128 ? 2 : 3) void attn_dkv_ke
   auto issue = [&](int t) {
     const unsigned to = lds0 + (t & 1) * 2 * TB;
     const int rows = min(tok_end - it.begin - t * tpt, tpt) * p.group;
-    lq.issue(qp + (long)t * tpt * p.q.st, rows, to);
-    lg.issue(gp + (long)t * tpt * p.g.st, rows, to + TB);
+    lq.issue(qp, rows, 0, 0, to);
+    lg.issue(gp, rows, 0, 0, to + TB);
+    qp += tpt * p.q.st;
+    gp += tpt * p.g.st;
   };
   if (tiles > 0) {
     fetch(0);
@@ -847,10 +893,11 @@ bool longer(const Item& a, const Item& b) {
   return a.begin < b.begin;
 }
 
-bool view_ok(const View& t, long tokens, long heads, int dim) {
-  // 16-byte loads; a tile's offsets (64 tokens and the heads of a group) stay below 2^31
+bool view_ok(const View& t, long tokens, long heads, int dim, bool keys = false) {
+  // 16-byte loads; a tile's offsets (up to 128 tokens and the heads of a group) stay below 2^31
+  if (keys && tokens > 1 && t.st < 2 * dim) return false;
   return t.p && ((unsigned long)t.p & 15) == 0 && t.st >= 0 && t.sh >= 0 && t.st % 16 == 0 && t.sh % 16 == 0 && t.st < (1l << 40) && t.sh < (1l << 40) &&
-         64 * t.st + 32 * t.sh + dim * 2 < (1l << 31);
+         128 * t.st + 32 * t.sh + dim * 2 < (1l << 31);
 }
 
 unsigned clear_blocks(long rows, long heads, int dim) { return (unsigned)std::min<long>(1024, (rows * heads * dim * 2 + CLEAR_BYTES - 1) / CLEAR_BYTES); }
@@ -1060,7 +1107,7 @@ extern "C" int dh_attn_fwd(const void* q, int64_t q_st, int64_t q_sh, const void
   p.q = {(const char*)q, q_st * 2, q_sh * 2}; p.k = {(const char*)k, k_st * 2, k_sh * 2}; p.v = {(const char*)v, v_st * 2, v_sh * 2}; p.o = {(const char*)o, o_st * 2, o_sh * 2};
   const int dim = (int)info->head_dim;
   if ((info->ints && !plan) || !lse || ((unsigned long)o_low & 15) || !view_ok(p.q, q_rows, info->heads, dim) || !view_ok(p.o, q_rows, info->heads, dim)) return DH_ERR_ARG;
-  if (info->k_rows && (!view_ok(p.k, k_rows, info->kv_heads, dim) || !view_ok(p.v, k_rows, info->kv_heads, dim))) return DH_ERR_ARG;
+  if (info->k_rows && (!view_ok(p.k, k_rows, info->kv_heads, dim, true) || !view_ok(p.v, k_rows, info->kv_heads, dim, true))) return DH_ERR_ARG;
   if (info->n_slots && (!workspace || ((unsigned long)workspace & 15) || workspace_bytes < dh_attn_fwd_workspace_bytes(info))) return DH_ERR_WORKSPACE;
   p.low = (char*)o_low; p.lse = lse; p.part = (float*)workspace; p.n_slots = info->n_slots;
   p.kv_heads = (int)info->kv_heads; p.heads = (int)info->heads; p.group = p.heads / p.kv_heads; p.dim = dim; p.block = (int)info->causal_block;
@@ -1100,7 +1147,7 @@ extern "C" int dh_attn_bwd(const void* grad, int64_t g_st, int64_t g_sh, const v
   }
   if (rest_q && !view_ok(p.dq, q_rows, info->heads, dim)) return DH_ERR_ARG;
   if (rest_k && (!view_ok(p.dk, k_rows, info->kv_heads, dim) || !view_ok(p.dv, k_rows, info->kv_heads, dim))) return DH_ERR_ARG;
-  if (info->n_dkv && (!view_ok(p.k, k_rows, info->kv_heads, dim) || !view_ok(p.v, k_rows, info->kv_heads, dim) || !view_ok(p.dk, k_rows, info->kv_heads, dim) ||
+  if (info->n_dkv && (!view_ok(p.k, k_rows, info->kv_heads, dim, true) || !view_ok(p.v, k_rows, info->kv_heads, dim, true) || !view_ok(p.dk, k_rows, info->kv_heads, dim) ||
                       !view_ok(p.dv, k_rows, info->kv_heads, dim))) return DH_ERR_ARG;
   p.low = (char*)const_cast<void*>(o_low); p.lse = const_cast<float*>(lse); p.delta = (float*)workspace; p.part = (float*)workspace + delta_floats(info); p.n_slots = info->n_dkv_slots;
   p.kv_heads = (int)info->kv_heads; p.heads = (int)info->heads; p.group = p.heads / p.kv_heads; p.dim = dim; p.block = (int)info->causal_block;

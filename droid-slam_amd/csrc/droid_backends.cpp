@@ -814,9 +814,12 @@ int64_t head_stride(const torch::Tensor& t) { return t.size(1) > 1 ? t.stride(1)
 // what dh_attn_* can read in place: adjacent channels, 16-byte pieces, offsets of a tile below 2^31
 bool attn_view(const torch::Tensor& t) {
   return t.stride(2) == 1 && ((uintptr_t)t.data_ptr() & 15) == 0 && row_stride(t) % 8 == 0 && head_stride(t) % 8 == 0 &&
-         row_stride(t) < (1ll << 24) && 64 * row_stride(t) + 32 * head_stride(t) + t.size(2) < (1ll << 30);
+         row_stride(t) < (1ll << 24) && 128 * row_stride(t) + 32 * head_stride(t) + t.size(2) < (1ll << 30);
 }
-torch::Tensor attn_input(const torch::Tensor& t) { return t.numel() == 0 || attn_view(t) ? t : t.clone(at::MemoryFormat::Contiguous); }
+torch::Tensor attn_input(const torch::Tensor& t, bool keys = false) {
+  const bool ok = t.numel() == 0 || (attn_view(t) && !(keys && t.size(0) > 1 && t.stride(0) < t.size(2)));        // rows of keys must not overlap
+  return ok ? t : t.clone(at::MemoryFormat::Contiguous);
+}
 
 dh_attn_info attn_info(const torch::Tensor& info) {
   TORCH_CHECK(info.device().is_cpu() && info.scalar_type() == torch::kInt64 && info.is_contiguous() && info.numel() * 8 == (int64_t)sizeof(dh_attn_info),
@@ -870,7 +873,7 @@ std::vector<torch::Tensor> attention_forward(torch::Tensor q, torch::Tensor k, t
     at::assert_no_internal_overlap(o);
     at::assert_no_overlap(o, q); at::assert_no_overlap(o, k); at::assert_no_overlap(o, v);
   }
-  q = attn_input(q); k = attn_input(k); v = attn_input(v);
+  q = attn_input(q); k = attn_input(k, true); v = attn_input(v, true);
   const size_t wsb = dh_attn_fwd_workspace_bytes(&i);
   torch::Tensor ws = torch::empty({(int64_t)wsb}, q.options().dtype(torch::kUInt8));
   check_status(dh_attn_fwd(TOKEN_VIEW(q), TOKEN_VIEW(k), TOKEN_VIEW(v), TOKEN_VIEW(o), for_backward ? low.data_ptr() : nullptr, lse.data_ptr<float>(),
@@ -894,7 +897,7 @@ std::vector<torch::Tensor> attention_backward(torch::Tensor grad, torch::Tensor 
   const int dt = token_dtype(q, "q", false);
   TORCH_CHECK(scale > 0 && scale < 1e30, "attention_backward: scale must be positive");
   const c10::DeviceGuard guard(q.device());
-  q = attn_input(q); k = attn_input(k); v = attn_input(v); o = attn_input(o); grad = attn_input(grad);
+  q = attn_input(q); k = attn_input(k, true); v = attn_input(v, true); o = attn_input(o); grad = attn_input(grad);
   const bool gaps = i.k_total < i.k_rows;
   torch::Tensor dq = torch::empty(q.sizes(), q.options());
   torch::Tensor dk = gaps ? torch::zeros(k.sizes(), k.options()) : torch::empty(k.sizes(), k.options());

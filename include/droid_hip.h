@@ -474,7 +474,8 @@ int dh_reproject_ex(const float* poses, const float* disps, const float* intrins
 /* ------------------------------------------------------------------------------------------------
  * Softmax attention over packed sequences of tokens (keyframe feature maps, frame by frame, row by row), forward and backward.
  *   q, o, grad, dq [q_rows, heads, head_dim], k, v, dk, dv [k_rows, kv_heads, head_dim], DH_F16 or DH_BF16; *_st / *_sh = elements between
- *   tokens / heads (channels adjacent; bases 16-byte aligned, strides multiples of 8 and >= 0, 64 * st + 32 * sh below 2^30 elements).
+ *   tokens / heads (channels adjacent; bases 16-byte aligned, strides multiples of 8 and >= 0, 128 * st + 32 * sh below 2^30 elements; rows of k / v do
+ *   not overlap).
  *   heads % kv_heads == 0 and heads / kv_heads <= 32: query head h reads key head h / (heads / kv_heads).  head_dim a multiple of 8 up to 128.
  * Sequence n has q_len[n] consecutive rows of q (packed one behind the other from row 0 on) and k_len[n] consecutive rows of k / v from row
  * k_start[n] on (k_start NULL: packed as well).  Its token i sees its first e(i) keys: all k_len (causal_block 0), or

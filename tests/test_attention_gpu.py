@@ -101,6 +101,11 @@ def test_views_and_padding(dtype):
     odd = lambda t: torch.cat([t.new_zeros(1), t.reshape(-1)])[1:].view(t.shape)  # noqa: E731  (an address that is no multiple of 16)
     check(odd(q), odd(k), odd(v), odd(g))
     check(*[torch.stack([t, t], -1)[..., 0] for t in (q, k, v, g)])          # channels not adjacent
+    same = k[:1].expand(120, -1, -1)                                         # one row of keys seen by all tokens: its gradient is a sum
+    r0 = oa.attention(q[:100], same[:100], v[:100], lengths, block=1, grad=g[:100])
+    leaf = k[:1].detach().clone().requires_grad_()
+    (dk,) = torch.autograd.grad(at.packed_attention(q, leaf.expand(120, -1, -1), v, plan), leaf, g)
+    near(dk, r0["dk"].sum(0, keepdim=True), r0["dk_err"].sum(0, keepdim=True) + 100 * oa.half_step(dtype) * r0["dk"].abs().sum(0, keepdim=True), "dk of a broadcast row")
     one = k[:, :1].expand(-1, kv, -1)                                        # one key head read by all: its gradient is a sum
     r1 = oa.attention(q[:100], one[:100], v[:100], lengths, block=1, grad=g[:100])
     leaf = k[:, :1].detach().clone().requires_grad_()
