@@ -659,22 +659,25 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_dq_kernel(const Params p) {
     }
 }
 
-// dK, dV: one workgroup holds 128 keys of one key head (64 where head_dim <= 64: half as long a walk, see below), 32 a wave, and walks over the
-// rows (tokens x group) that see them, 32 (64, in two waves) rows a tile.
-// S = Q K^T and dP = dO V^T have one key per lane, so P and dS are B operands of dV^T = dO^T P and dK^T = Q^T dS.  K stays in registers; V
-// does not fit next to the two accumulators (with it the 128-channel form spilled: 6.0 ms instead of the figure below) and is read from LDS.
+// dK, dV: one workgroup holds 64 keys of one key head (128 where head_dim > 64), 32 a wave, and walks over the rows (tokens x group) that see
+// them, 64 rows a tile, 32 a wave: 4 (8) waves, the two halves of the rows meet at the end.
+// S = Q K^T and dP = dO V^T have one key per lane, so P and dS are B operands of dV^T = dO^T P and dK^T = Q^T dS.
+// What bounds it is the wait for LDS operands, which a wave can only read ahead into registers it has: at 128 channels the two accumulators are
+// 128 of 256.  With K and V in registers the kernel spilled (training window of 12 x 1200 tokens: 6.0 ms), with V in LDS it had no room to
+// read ahead (2.1 ms), with both in LDS, a tile serving 8 waves, it takes 1.87 ms.  64 keys a wave (half the LDS reads, one wave a SIMD) spilled.
 // slot >= 0: the walk over the rows is split, 32-bit sums go to the workspace for attn_dkv_join.
-constexpr int DKV_WAVES = 4;
 template <int DP> struct Dkv {
-  static constexpr int KW = DP == 128 ? 4 : 2, RW = DKV_WAVES / KW;          // waves along the keys / along the rows
-  static constexpr int KEYS = KW * 32, ROWS = RW * 32, TB = ROWS * Geo<DP>::ROWB;
-  static constexpr int LDS = 4 * TB + KEYS * Geo<DP>::ROWB + 5 * ROWS * 4;
+  static constexpr bool WIDE = DP == 128;                                    // K in LDS as well
+  static constexpr int KW = WIDE ? 4 : 2, RW = 2;                            // waves along the keys / along the rows
+  static constexpr int WAVES = KW * RW, KEYS = KW * 32, ROWS = RW * 32, TB = ROWS * Geo<DP>::ROWB;
+  static constexpr int LDS = 4 * TB + (WIDE ? 2 : 1) * KEYS * Geo<DP>::ROWB + 5 * ROWS * 4;
 };
 
 template <typename T, int DP>
-__global__ __launch_bounds__(DKV_WAVES * 64, DP == 128 ? 2 : 3) void attn_dkv_kernel(const Params p) {
+__global__ __launch_bounds__(Dkv<DP>::WAVES * 64, DP == 128 ? 2 : 3) void attn_dkv_kernel(const Params p) {
   using G = Geo<DP>;
-  constexpr int TB = Dkv<DP>::TB, DKV_ROWS = Dkv<DP>::ROWS, DKV_KEYS = Dkv<DP>::KEYS;
+  constexpr int TB = Dkv<DP>::TB, DKV_ROWS = Dkv<DP>::ROWS, DKV_KEYS = Dkv<DP>::KEYS, DKV_WAVES = Dkv<DP>::WAVES;
+  constexpr bool WIDE = Dkv<DP>::WIDE;
   extern __shared__ __attribute__((aligned(1024))) char dyn[];               // [buffer][Q, dO], V, [buffer][lse2, delta], tokens of the rows
   const int lane = threadIdx.x & 63, wave = (threadIdx.x >> 6) % Dkv<DP>::KW, rw = (threadIdx.x >> 6) / Dkv<DP>::KW;       // 32 keys, 32 rows of a tile
   if (blockIdx.x >= p.blocks) {
@@ -688,7 +691,7 @@ __global__ __launch_bounds__(DKV_WAVES * 64, DP == 128 ? 2 : 3) void attn_dkv_ke
   const int key = it.first + wave * 32 + (lane & 31);
   const bool valid = key < it.k_len;
   char* const vtile = dyn + 4 * TB;
-  float* const stat = reinterpret_cast<float*>(vtile + DKV_KEYS * G::ROWB);
+  float* const stat = reinterpret_cast<float*>(vtile + (WIDE ? 2 : 1) * DKV_KEYS * G::ROWB);
   int* const row_tok = reinterpret_cast<int*>(stat + 4 * DKV_ROWS);
   lds_char* const lds = (lds_char*)dyn;
   const unsigned lds0 = (unsigned)(unsigned long)lds;
@@ -696,6 +699,10 @@ __global__ __launch_bounds__(DKV_WAVES * 64, DP == 128 ? 2 : 3) void attn_dkv_ke
     TileLoader<DP, DKV_WAVES, DKV_KEYS, true> l;
     l.init(p.v, p.dim, 1, DKV_KEYS);
     l.issue(p.v.p + uniform((long)(it.k_start + it.first) * p.v.st + (long)hk * p.v.sh), it.k_len - it.first, (unsigned)p.v.st, p.dim * 2, lds0 + 4 * TB);
+    if (WIDE) {
+      l.init(p.k, p.dim, 1, DKV_KEYS);
+      l.issue(p.k.p + uniform((long)(it.k_start + it.first) * p.k.st + (long)hk * p.k.sh), it.k_len - it.first, (unsigned)p.k.st, p.dim * 2, lds0 + 4 * TB + DKV_KEYS * G::ROWB);
+    }
   }
   u32x4 kf[DP / 16];
   {
@@ -772,7 +779,8 @@ __global__ __launch_bounds__(DKV_WAVES * 64, DP == 128 ? 2 : 3) void attn_dkv_ke
       for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.f;
 #pragma unroll
       for (int ks = 0; ks < DP / 16; ++ks) {
-        s = T::mfma(frag<DP>(qt, rw, ks, lane), kf[ks], s);
+        if constexpr (WIDE) s = T::mfma(frag<DP>(qt, rw, ks, lane), frag<DP>(vt + DKV_KEYS * G::ROWB, wave, ks, lane), s);
+        else s = T::mfma(frag<DP>(qt, rw, ks, lane), kf[ks], s);
         dp = T::mfma(frag<DP>(gt, rw, ks, lane), frag<DP>(vt, wave, ks, lane), dp);
       }
       const bool masked = first_tok < wave_all;
@@ -935,7 +943,7 @@ template <typename T, int DP> int run_bwd(Params p, const dh_attn_info& info, co
   more = clear_blocks(p.k_rows - p.clear_k, p.kv_heads, p.dim);
   if (p.blocks + more) {
     DH_LDS_OPTIN((attn_dkv_kernel<T, DP>), Dkv<DP>::LDS);
-    hipLaunchKernelGGL((attn_dkv_kernel<T, DP>), dim3(p.blocks + more), dim3(DKV_WAVES * 64), Dkv<DP>::LDS, st, p);
+    hipLaunchKernelGGL((attn_dkv_kernel<T, DP>), dim3(p.blocks + more), dim3(Dkv<DP>::WAVES * 64), Dkv<DP>::LDS, st, p);
     DH_LAUNCH_CHECK();
   }
   p.items += info.n_dkv;
@@ -992,8 +1000,9 @@ extern "C" int dh_attn_plan(const int64_t* q_len, const int64_t* k_len, const in
       if (n <= slots_on_chip || longest <= piece) break;
       piece += std::max<long>(1, piece / 16);
     }
-  // the same for the rows of dK and dV: a split key tile costs a trip of its sums through memory (a quarter of a millisecond's work for all
-  // of them at most), so pieces are 64 tiles of 32 rows at least
+  // The same for the rows of dK and dV.  A split key tile costs a trip of its 32-bit sums through memory, so pieces are 24 tiles of 64 rows at
+  // least.  One share a place where three workgroups fit a CU; four where one does (training window, 128 channels: 3.20, 3.09, 3.04 ms with two,
+  // one, four shares of 256; packed clips, 64 channels: 124, 121 us with two, one share of 768).
   long row_tiles = 0;
   auto rows_of = [&](int64_t i, long x) -> long {              // the first token that sees key x
     return block ? std::min<long>(q_len[i], std::max<long>(0, x / block * block - (k_len[i] - q_len[i]))) : 0;
@@ -1002,7 +1011,7 @@ extern "C" int dh_attn_plan(const int64_t* q_len, const int64_t* k_len, const in
   const int dkv_keys = wide ? Dkv<128>::KEYS : Dkv<64>::KEYS, tpt_k = (wide ? Dkv<128>::ROWS : Dkv<64>::ROWS) / group;
   for (int64_t i = 0; i < n_seqs; ++i)
     for (long x = 0; x < k_len[i]; x += dkv_keys) row_tiles += (q_len[i] - rows_of(i, x) + tpt_k - 1) / tpt_k * (long)kv_heads;
-  const long piece_k = std::max<long>(64, (row_tiles + 1023) / 1024);
+  const long shares = wide ? 1024 : 768, piece_k = std::max<long>(24, (row_tiles + shares - 1) / shares);
   Item* base = reinterpret_cast<Item*>(plan);
   const long cap = plan ? plan_ints / 8 : 0;
   Writer w{base, cap, 0};
@@ -1041,7 +1050,7 @@ extern "C" int dh_attn_plan(const int64_t* q_len, const int64_t* k_len, const in
           const int t0 = (int)rows_of(i, x);
           Item it{(int)qs, m, ks, n, x, t0, m, -1};
           const long nt = ((long)m - t0 + tpt_k - 1) / tpt_k;
-          const long pieces = nt > piece_k + piece_k / 2 ? (nt + piece_k - 1) / piece_k : 1;
+          const long pieces = nt > piece_k + piece_k / 4 ? (nt + piece_k - 1) / piece_k : 1;
           if (pass == 3 && pieces == 1) w.put(it);
           else if (pass == 3) {
             for (long y = 0; y < pieces; ++y) {

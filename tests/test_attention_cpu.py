@@ -31,11 +31,12 @@ PLANS = [([1], None, 1, 1, 0), ([48], None, 4, 4, 0), ([5, 0, 300, 1], None, 8, 
          ([1] * 9, [1, 0, 63, 64, 65, 5000, 9000, 129, 20000], 16, 2, 1), ([2000], [500], 4, 4, 7), ([700], [9000], 3, 1, 0), ([9000], [40], 8, 1, 0), ([6000], None, 16, 2, 100), ([], None, 4, 2, 0)]
 
 
+@pytest.mark.parametrize("dim,keys_a_tile", [(64, 64), (128, 128)])
 @pytest.mark.parametrize("lengths,key_lengths,heads,kv_heads,block", PLANS)
-def test_plan_covers_every_row_and_key_once(lengths, key_lengths, heads, kv_heads, block):
+def test_plan_covers_every_row_and_key_once(lengths, key_lengths, heads, kv_heads, block, dim, keys_a_tile):
     """each visible (row, key) pair is in exactly one forward item, one dQ item and one dK / dV item"""
     keys = lengths if key_lengths is None else key_lengths
-    info, (fwd, join, dq, dkv, dkv_join) = plan(lengths, heads, kv_heads, 64, key_lengths=key_lengths, causal_block=block)
+    info, (fwd, join, dq, dkv, dkv_join) = plan(lengths, heads, kv_heads, dim, key_lengths=key_lengths, causal_block=block)
     assert info["q_rows"] == sum(lengths) and info["k_rows"] == sum(keys) == info["k_total"] and not info["keys_shared"]
     group = heads // kv_heads
     q0 = k0 = 0
@@ -54,7 +55,7 @@ def test_plan_covers_every_row_and_key_once(lengths, key_lengths, heads, kv_head
         for qs, ql, ks, kl, first, begin, end, _ in dkv:
             if (qs, ql) == (q0, m) and (ks, kl) == (k0, l) and l:
                 assert 0 <= begin <= end <= m
-                hit[begin:end, first:first + 64] += 1
+                hit[begin:end, first:first + keys_a_tile] += 1
         assert bool((hit[seen] == 1).all()) and bool((hit <= 1).all())
         q0, k0 = q0 + m, k0 + l
     slots = sorted(x for j in join for x in range(j[5], j[5] + j[6]))
