@@ -956,7 +956,7 @@ template <typename T, int DP> int run_bwd(Params p, const dh_attn_info& info, co
 
 bool info_ok(const dh_attn_info* i) {
   return i && heads_ok(i->heads, i->kv_heads, i->head_dim) && i->causal_block >= 0 && i->causal_block <= MAX_ROWS && (i->waves == 1 || i->waves == 4) &&
-         i->n_fwd >= 0 && i->n_join >= 0 && i->n_dq >= 0 && i->n_dkv >= 0 && i->n_dkv_join >= 0 && i->n_slots >= 0 && i->n_dkv_slots >= 0 && i->q_rows >= 0 && i->k_rows >= 0 && i->q_rows <= MAX_ROWS && i->k_rows <= MAX_ROWS &&
+         i->ints == 8 * (i->n_fwd + i->n_join + i->n_dq + i->n_dkv + i->n_dkv_join) && i->n_fwd >= 0 && i->n_join >= 0 && i->n_dq >= 0 && i->n_dkv >= 0 && i->n_dkv_join >= 0 && i->n_slots >= 0 && i->n_dkv_slots >= 0 && i->q_rows >= 0 && i->k_rows >= 0 && i->q_rows <= MAX_ROWS && i->k_rows <= MAX_ROWS &&
          i->n_fwd * i->kv_heads <= INT_MAX - 1024 && i->n_join * i->kv_heads <= 65535 && i->n_dq * i->kv_heads <= INT_MAX - 1024 && i->n_dkv * i->kv_heads <= INT_MAX - 1024 && i->n_dkv_join * i->kv_heads <= 65535;
 }
 
@@ -982,7 +982,7 @@ extern "C" int dh_attn_plan(const int64_t* q_len, const int64_t* k_len, const in
   const int tpt = waves * 32 / group, tpt_q = 128 / group;
   // Long walks over the keys become several work items (pieces of whole key tiles, joined afterwards) where they would outlast the rest:
   // the aim is an equal share of all key tiles for each of the workgroups that the chip holds at once.  A walk is only split if that saves
-  // 8 tiles: a split row's sums go through memory once more, and the join is a launch of its own.
+  // 24 tiles (some 20 us): a split row's sums go through memory once more, and the join is a launch of its own.
   const int dp = pad_dim(head_dim), slots_on_chip = 256 * (waves == 1 ? (dp == 128 ? 3 : 6) : dp == 128 ? 2 : 3);       // LDS or registers hold no more
   const int64_t* ql = q_len; const int64_t* kl = k_len;
   auto each_tile = [&](auto&& f) {
@@ -992,7 +992,7 @@ extern "C" int dh_attn_plan(const int64_t* q_len, const int64_t* k_len, const in
   long tiles = 0, walks = 0;
   each_tile([&](long nt) { tiles += nt * kv_heads; walks += kv_heads; });
   long piece = std::max<long>(4, (tiles + slots_on_chip - 1) / slots_on_chip);
-  auto pieces_of = [&](long nt) -> long { return nt > piece + piece / 8 + 8 ? (nt + piece - 1) / piece : 1; };
+  auto pieces_of = [&](long nt) -> long { return nt > piece + piece / 8 + 24 ? (nt + piece - 1) / piece : 1; };
   if (walks < slots_on_chip)                     // rounding up must not leave a few items for a second round
     for (;;) {
       long n = 0, longest = 0;

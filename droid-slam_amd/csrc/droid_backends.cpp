@@ -11,6 +11,7 @@
 #include <c10/hip/HIPStream.h>
 #include <c10/core/DeviceGuard.h>
 #include <ATen/MemoryOverlap.h>
+#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <vector>
 #include <algorithm>
 #include "../../include/droid_hip.h"
@@ -854,6 +855,7 @@ void check_attn(const torch::Tensor& q, const torch::Tensor& k, const torch::Ten
   TORCH_CHECK(q.size(0) >= i.q_rows, what, ": the plan has ", i.q_rows, " query rows, q has ", q.size(0));
   TORCH_CHECK(k.size(0) >= i.k_rows, what, ": the plan has ", i.k_rows, " key rows, k has ", k.size(0));
   TORCH_CHECK(plan.device() == q.device() && plan.scalar_type() == torch::kInt32 && plan.is_contiguous() && plan.numel() == i.ints, what, ": the plan is on another device");
+  plan.record_stream(c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(q.get_device()).unwrap());       // the caller may drop a plan while its work is queued, on any stream
 }
 
 // {o [rows, heads, head_dim], lse [rows, heads] f32, o_low (for_backward: what the rounding of o left behind; else empty)}; rows behind the last sequence are 0 / -inf, or left alone in an `out` of the caller's

@@ -27,7 +27,7 @@ class PackedPlan:
     key_starts     first key row of each sequence (default: packed one behind the other), e.g. the slots of a cache
 
     Query rows are packed one behind the other from row 0 on.  The plan belongs to its lengths, heads, head_dim and device; it may be used
-    by any number of calls, also at once on several streams and in captured graphs."""
+    by any number of calls, also at once on several streams, and in captured graphs (which it has to outlive)."""
 
     def __init__(self, lengths, heads, kv_heads, head_dim, key_lengths=None, causal_block=0, key_starts=None, device="cuda"):
         lengths = [int(n) for n in lengths]

@@ -312,6 +312,44 @@ def test_captured_training_step():
         assert all(torch.equal(a, b) for a, b in zip(out, want[i % 2])), i
 
 
+def test_offsets_beyond_32_bits():
+    """rows that lie more than 4 GiB from the start: far slots of a cache, and token strides of 16 MB"""
+    h, kv, d, far = 4, 2, 64, 20000000
+    cache = [torch.empty(far + 300, kv, d, dtype=BF16, device="cuda") for _ in range(2)]
+    assert far * kv * d * 2 > 1 << 32
+    q, k, v, g = inputs([5, 200], [5, 300], h, kv, d, BF16, 50)
+    for c, t in zip(cache, (k, v)):
+        c[:5], c[far:] = t[:5], t[5:]
+    plan = at.PackedPlan([5, 200], h, kv, d, key_lengths=[5, 300], key_starts=[0, far], causal_block=1)
+    r = oa.attention(q, k, v, [5, 200], [5, 300], block=1, grad=g)
+    leaves = [q.clone().requires_grad_()] + [c.requires_grad_() for c in cache]
+    o = at.packed_attention(*leaves, plan)
+    near(o, r["o"], r["o_err"], "o")
+    grads = torch.autograd.grad(o, leaves, g)
+    near(grads[0], r["dq"], r["dq_err"], "dq")
+    for n, t in zip(("dk", "dv"), grads[1:]):
+        near(torch.cat([t[:5], t[far:]]), r[n], r[n + "_err"], n)
+        assert not t[5:200].any()
+    del cache, leaves, grads
+    n, st = 330, 8000000                                                     # elements between tokens
+    assert n * st * 2 > 1 << 32
+    wide = torch.empty(n * st, dtype=BF16, device="cuda")
+    lay = lambda t, at_: wide.as_strided(t.shape, (st, t.shape[2], 1), at_).copy_(t)  # noqa: E731
+    q, k, v, g = inputs([n], None, h, kv, d, BF16, 60)
+    r = oa.attention(q, k, v, [n], block=1, grad=g)
+    Q, K, V, G = lay(q, 0), lay(k, 1024), lay(v, 2048), lay(g, 4096)
+    plan = at.PackedPlan([n], h, kv, d, causal_block=1)
+    out = wide.as_strided(q.shape, (st, d, 1), 8192)
+    near(at.packed_attention(Q, K, V, plan, out=out), r["o"], r["o_err"], "o")
+    leaves = [t.detach().requires_grad_() for t in (Q, K, V)]
+    for name, t in zip(("dq", "dk", "dv"), torch.autograd.grad(at.packed_attention(*leaves, plan), leaves, G)):
+        near(t, r[name], r[name + "_err"], name)
+    pos, fr = torch.arange(n).int().cuda(), torch.rand(32).cuda()
+    rq = oa.qk_norm_rope(q, pos, fr, [32], grad=g)
+    y = at.qk_norm_rope(Q, K, pos, fr, [32], out=(out, wide.as_strided(k.shape, (st, d, 1), 16384)))
+    near(y[0], rq["y"], rq["y_err"], "rotation")
+
+
 def test_attention_refusals():
     plan = at.PackedPlan([8], 4, 2, 64)
     q, k, v, g = inputs([8], None, 4, 2, 64, F16)
@@ -327,6 +365,10 @@ def test_attention_refusals():
     leaf = q.clone().requires_grad_()
     with pytest.raises(RuntimeError, match="once"):
         torch.autograd.grad(at.packed_attention(leaf, k, v, plan), leaf, g, create_graph=True)
+    other = at.PackedPlan([8, 3], 4, 2, 64)
+    for info, items in ((other.info, plan.items), (plan.info, other.items), (plan.info[:-1], plan.items), (plan.info.cuda(), plan.items), (torch.zeros_like(plan.info), plan.items)):
+        with pytest.raises(RuntimeError):
+            at.droid_backends.attention_forward(q, k, v, items, info, 0.1)
     empty = at.PackedPlan([], 4, 2, 64)
     assert not at.packed_attention(q, k, v, empty).any()
     assert at.packed_attention(q[:0], k[:0], v[:0], empty).shape == (0, 4, 64)
