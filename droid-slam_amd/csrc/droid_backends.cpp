@@ -10,6 +10,7 @@
 #include <torch/extension.h>
 #include <c10/hip/HIPStream.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <ATen/MemoryOverlap.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <vector>
@@ -911,6 +912,19 @@ std::vector<torch::Tensor> attention_backward(torch::Tensor grad, torch::Tensor 
   return {dq, dk, dv};
 }
 
+// A leaf keeps the stream that its gradient was first wanted on for as long as a graph of it lives; autograd would join that stream into a
+// capture, which ends the process.  Refused instead, before anything is recorded.
+void refuse_leaves_of_other_streams(std::initializer_list<const torch::Tensor*> inputs, const char* what) {
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+  for (const torch::Tensor* t : inputs) {
+    if (!t || !t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+    const auto stream = node ? node->stream() : c10::nullopt;
+    TORCH_CHECK(!stream || *stream == c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t->get_device()).unwrap(), what,
+                ": this stream is being captured, and a graph of the same leaves lives on another one; drop it first");
+  }
+}
+
 // the same with a gradient (once): what droid_amd.attention.packed_attention calls where one is wanted
 struct PackedAttention : public torch::autograd::Function<PackedAttention> {
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor plan, torch::Tensor info,
@@ -929,6 +943,7 @@ struct PackedAttention : public torch::autograd::Function<PackedAttention> {
   }
 };
 std::vector<torch::Tensor> packed_attention(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor plan, torch::Tensor info, double scale) {
+  refuse_leaves_of_other_streams({&q, &k, &v}, "packed_attention");
   return PackedAttention::apply(q, k, v, plan, info, scale);
 }
 
@@ -1042,6 +1057,7 @@ struct QkNormRope : public torch::autograd::Function<QkNormRope> {
 };
 std::vector<torch::Tensor> qk_norm_rope(torch::Tensor q, torch::Tensor k, torch::Tensor positions, torch::Tensor inv_freq, const std::vector<int64_t>& sections,
                                         c10::optional<torch::Tensor> q_weight, c10::optional<torch::Tensor> k_weight, bool normalize, double eps, bool interleaved) {
+  refuse_leaves_of_other_streams({&q, &k, q_weight ? &*q_weight : nullptr, k_weight ? &*k_weight : nullptr}, "qk_norm_rope");
   return QkNormRope::apply(q, k, positions, inv_freq, q_weight, k_weight, sections, normalize, eps, interleaved);
 }
 

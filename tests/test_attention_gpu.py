@@ -312,6 +312,27 @@ def test_captured_training_step():
         assert all(torch.equal(a, b) for a, b in zip(out, want[i % 2])), i
 
 
+def test_capture_beside_a_living_graph_of_the_same_leaves_is_refused():
+    q, k, v, g = inputs([40], None, 4, 2, 64, BF16)
+    plan = at.PackedPlan([40], 4, 2, 64, causal_block=1)
+    pos, fr = torch.arange(40, device="cuda", dtype=torch.int32), torch.rand(32, device="cuda")
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    alive = at.packed_attention(*leaves, plan)
+    for call in (lambda: at.packed_attention(*leaves, plan), lambda: at.qk_norm_rope(leaves[0], leaves[1], pos, fr, [32])):
+        with pytest.raises(RuntimeError, match="captured"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                call()
+    want = torch.autograd.grad(alive, leaves, g)
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(at.packed_attention(*leaves, plan), leaves, g)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_offsets_beyond_32_bits():
     """rows that lie more than 4 GiB from the start: far slots of a cache, and token strides of 16 MB"""
     h, kv, d, far = 4, 2, 64, 20000000
