@@ -982,7 +982,9 @@ extern "C" int dh_attn_plan(const int64_t* q_len, const int64_t* k_len, const in
   const int tpt = waves * 32 / group, tpt_q = 128 / group;
   // Long walks over the keys become several work items (pieces of whole key tiles, joined afterwards) where they would outlast the rest:
   // the aim is an equal share of all key tiles for each of the workgroups that the chip holds at once.  A walk is only split if that saves
-  // 24 tiles (some 20 us): a split row's sums go through memory once more, and the join is a launch of its own.
+  // 24 tiles (some 20 us) of a workgroup's walk: a split row's sums go through memory once more, and the join is a launch of its own (packed clips,
+  // 64 channels: 87 us with 8, 85 with 24).  Lone waves are split for any saving: long walks meet short ones there, and a join is needed anyway (32
+  // queries over 1 .. 32400 keys: 82 us; 87 if it had to save 4 tiles, 130 if 24).
   const int dp = pad_dim(head_dim), slots_on_chip = 256 * (waves == 1 ? (dp == 128 ? 3 : 6) : dp == 128 ? 2 : 3);       // LDS or registers hold no more
   const int64_t* ql = q_len; const int64_t* kl = k_len;
   auto each_tile = [&](auto&& f) {
@@ -992,7 +994,7 @@ extern "C" int dh_attn_plan(const int64_t* q_len, const int64_t* k_len, const in
   long tiles = 0, walks = 0;
   each_tile([&](long nt) { tiles += nt * kv_heads; walks += kv_heads; });
   long piece = std::max<long>(4, (tiles + slots_on_chip - 1) / slots_on_chip);
-  auto pieces_of = [&](long nt) -> long { return nt > piece + piece / 8 + 24 ? (nt + piece - 1) / piece : 1; };
+  auto pieces_of = [&](long nt) -> long { return nt > piece + piece / 8 + (waves == 1 ? 0 : 24) ? (nt + piece - 1) / piece : 1; };
   if (walks < slots_on_chip)                     // rounding up must not leave a few items for a second round
     for (;;) {
       long n = 0, longest = 0;

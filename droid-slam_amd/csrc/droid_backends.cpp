@@ -859,7 +859,7 @@ void check_attn(const torch::Tensor& q, const torch::Tensor& k, const torch::Ten
   plan.record_stream(c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(q.get_device()).unwrap());       // the caller may drop a plan while its work is queued, on any stream
 }
 
-// {o [rows, heads, head_dim], lse [rows, heads] f32, o_low (for_backward: what the rounding of o left behind; else empty)}; rows behind the last sequence are 0 / -inf, or left alone in an `out` of the caller's
+// {o [rows, heads, head_dim], lse [rows, heads] f32, o_low (for_backward: what the rounding of o left behind; else None)}; rows behind the last sequence are 0 / -inf, or left alone in an `out` of the caller's
 std::vector<torch::Tensor> attention_forward(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor plan, torch::Tensor info, double scale,
                                              c10::optional<torch::Tensor> out, bool for_backward) {
   const dh_attn_info i = attn_info(info);
@@ -869,7 +869,7 @@ std::vector<torch::Tensor> attention_forward(torch::Tensor q, torch::Tensor k, t
   const c10::DeviceGuard guard(q.device());
   torch::Tensor o = out ? *out : torch::empty(q.sizes(), q.options());
   torch::Tensor lse = torch::empty({q.size(0), q.size(1)}, q.options().dtype(torch::kFloat32));
-  torch::Tensor low = for_backward ? torch::empty(q.sizes(), q.options()) : torch::empty({0}, q.options());
+  torch::Tensor low = for_backward ? torch::empty(q.sizes(), q.options()) : torch::Tensor();
   if (out) {
     check_heads(o, "out", q);
     TORCH_CHECK(o.sizes() == q.sizes() && attn_view(o), "out must have q's shape, adjacent channels and 16-byte aligned heads");
@@ -878,9 +878,10 @@ std::vector<torch::Tensor> attention_forward(torch::Tensor q, torch::Tensor k, t
   }
   q = attn_input(q); k = attn_input(k, true); v = attn_input(v, true);
   const size_t wsb = dh_attn_fwd_workspace_bytes(&i);
-  torch::Tensor ws = torch::empty({(int64_t)wsb}, q.options().dtype(torch::kUInt8));
+  torch::Tensor ws;
+  if (wsb) ws = torch::empty({(int64_t)wsb}, q.options().dtype(torch::kUInt8));
   check_status(dh_attn_fwd(TOKEN_VIEW(q), TOKEN_VIEW(k), TOKEN_VIEW(v), TOKEN_VIEW(o), for_backward ? low.data_ptr() : nullptr, lse.data_ptr<float>(),
-                           plan.data_ptr<int32_t>(), &i, dt, q.size(0), k.size(0), (float)scale, !out, ws.data_ptr(), wsb, stream_of(q)), "attention_forward");
+                           plan.data_ptr<int32_t>(), &i, dt, q.size(0), k.size(0), (float)scale, !out, wsb ? ws.data_ptr() : nullptr, wsb, stream_of(q)), "attention_forward");
   if (out && q.size(0) > i.q_rows) lse.narrow(0, i.q_rows, q.size(0) - i.q_rows).fill_(-std::numeric_limits<float>::infinity());
   return {o, lse, low};
 }
@@ -1010,7 +1011,7 @@ std::vector<torch::Tensor> qk_norm_rope_forward(torch::Tensor q, torch::Tensor k
   return {qo, ko};
 }
 
-// {dq, dk, dq_weight, dk_weight}; the weights' gradients are empty where there is no weight
+// {dq, dk, dq_weight, dk_weight}; the weights' gradients are None where there is no weight
 std::vector<torch::Tensor> qk_norm_rope_backward(torch::Tensor dq_out, torch::Tensor dk_out, torch::Tensor q, torch::Tensor k, torch::Tensor positions, torch::Tensor inv_freq,
                                                  const std::vector<int64_t>& sections, c10::optional<torch::Tensor> q_weight, c10::optional<torch::Tensor> k_weight,
                                                  bool normalize, double eps, bool interleaved) {
@@ -1021,12 +1022,14 @@ std::vector<torch::Tensor> qk_norm_rope_backward(torch::Tensor dq_out, torch::Te
   const c10::DeviceGuard guard(q.device());
   q = rope_input(q); k = rope_input(k); dq_out = rope_input(dq_out); dk_out = rope_input(dk_out);
   torch::Tensor dq = torch::empty(q.sizes(), q.options()), dk = torch::empty(k.sizes(), k.options());
-  torch::Tensor dqw = q_weight ? torch::empty_like(*q_weight) : torch::empty({0}, q.options()), dkw = k_weight ? torch::empty_like(*k_weight) : torch::empty({0}, q.options());
+  torch::Tensor dqw, dkw, ws;
+  if (q_weight) dqw = torch::empty_like(*q_weight);
+  if (k_weight) dkw = torch::empty_like(*k_weight);
   const size_t wsb = q_weight || k_weight ? dh_qk_norm_rope_bwd_workspace_bytes((int)q.size(2)) : 0;
-  torch::Tensor ws = torch::empty({(int64_t)wsb}, q.options().dtype(torch::kUInt8));
+  if (wsb) ws = torch::empty({(int64_t)wsb}, q.options().dtype(torch::kUInt8));
   rope_status(dh_qk_norm_rope_bwd(TOKEN_VIEW(dq_out), TOKEN_VIEW(dk_out), TOKEN_VIEW(q), TOKEN_VIEW(k), TOKEN_VIEW(dq), TOKEN_VIEW(dk), q_weight ? dqw.data_ptr() : nullptr,
                                   k_weight ? dkw.data_ptr() : nullptr, positions.data_ptr(), a.pos_type, inv_freq.data_ptr<float>(), a.sections.data(), (int)a.sections.size(),
-                                  a.qw, a.kw, a.w_dtype, dt, q.size(0), (int)q.size(1), (int)k.size(1), (int)q.size(2), normalize, (float)eps, interleaved, ws.data_ptr(), wsb,
+                                  a.qw, a.kw, a.w_dtype, dt, q.size(0), (int)q.size(1), (int)k.size(1), (int)q.size(2), normalize, (float)eps, interleaved, wsb ? ws.data_ptr() : nullptr, wsb,
                                   stream_of(q)), "qk_norm_rope_backward");
   return {dq, dk, dqw, dkw};
 }
