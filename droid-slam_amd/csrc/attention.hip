@@ -78,7 +78,7 @@ struct BF16 {
 constexpr int BN = 64;                           // rows of an LDS tile
 constexpr unsigned OUT_OF_RANGE = 0x80000000u;   // byte offset behind every buffer: such lanes of an LDS-DMA write zeros
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
-constexpr float M_FLOOR = -1e30f;                // start of the running maximum: finite, so that a row without keys makes no inf - inf
+constexpr float M_FLOOR = -3e38f;                // start of the running maximum: finite, so that a row without keys makes no inf - inf
 
 struct Item { int q_start, q_len, k_start, k_len, first, begin, end, slot; };   // the plan's record, see dh_attn_plan
 
@@ -215,7 +215,7 @@ __host__ __device__ __forceinline__ int keys_seen(int i, int q_len, int k_len, i
   return e < (unsigned)k_len ? (int)e : k_len;
 }
 
-__device__ __forceinline__ bool item_ok(const Item& it, const Params& p) {   // never true of a plan of dh_attn_plan for these tensors
+__device__ __forceinline__ bool item_ok(const Item& it, const Params& p) {   // (holds for a plan of dh_attn_plan with these tensors)
   return it.q_start >= 0 && it.q_len >= 0 && it.k_start >= 0 && it.k_len >= 0 && it.first >= 0 && it.begin >= 0 &&
          (long)it.q_start + it.q_len <= p.q_rows && (long)it.k_start + it.k_len <= p.k_rows;
 }
@@ -267,8 +267,10 @@ constexpr int CLEAR_BYTES = 1 << 15;             // a workgroup's share
 // One workgroup: NW x 32 rows (NW * 32 / group tokens) of one key head over the keys [begin, end) of its sequence.  Running maximum and sum
 // per row; the accumulator is only rescaled when a maximum grew by more than 2^8 (p <= 256 until then: exact in 32 bits, and a 16-bit p
 // keeps its relative precision).  slot >= 0: the row range is split over the keys, unnormalised sums go to the workspace for attn_join.
-// How the keys come in: 64 keys a tile, one tile ahead; a lone wave (few rows, bound by memory) takes 32 and keeps two
-// tiles on their way in 48 KB, three waves a CU (32 queries over 358 MB of keys: 90 us; two or four stages with as many waves as fit 99 and 95).
+// Bound by the matrix cores at the power limit (128 channels: 1.11 PFLOP/s on 19200 tokens, the library's large product 1.25), by the vector
+// units at 64 channels (0.72 on packed clips).
+// How the keys come in: 64 keys a tile, one tile ahead; a lone wave (few rows, bound by memory: 82 us for 32 queries over 358 MB of keys, 4.4 TB/s)
+// takes 32 and keeps two tiles on their way in 48 KB, three waves a CU (90 us; with the same plan, two or four stages and as many waves as fit: 99, 95).
 template <int NW> struct Walk { static constexpr int BLOCKS = NW == 1 ? 1 : 2, STAGES = NW == 1 ? 3 : 2; };
 
 template <typename T, int DP, int NW>
@@ -291,7 +293,7 @@ __global__ __launch_bounds__(NW * 64, NW == 1 ? 1 : DP == 128 ? 2 : 3) void attn
   const bool valid = row < tpt * p.group && tok < it.q_len;
   const int key_end = min(it.end, it.k_len);
   const int lim = valid ? min(keys_seen(tok, it.q_len, it.k_len, p.block), key_end) : key_end;
-  const int wmin = wave_min(lim), wmax = wave_max(valid ? lim : 0);
+  const int wmin = wave_min(lim);
 
   u32x4 qf[DP / 16];
   {
@@ -545,7 +547,8 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const Params p, int rows
 
 // ------------------------------------------------------------------------------------------------------------ backward
 // dQ: the forward's walk over the keys with dO next to Q.  S^T and dP^T = V dO^T give dS^T in the layout of a B operand; the K tile is
-// read a second time transposed for dQ^T = K^T dS^T.  Writes delta for attn_dkv_kernel on the way.
+// read a second time transposed for dQ^T = K^T dS^T.  Writes delta for attn_dkv_kernel on the way.  Split as the forward is; 1.18 PFLOP/s on a
+// training window of 14400 tokens (128 channels).
 template <typename T, int DP, int NW>
 __global__ __launch_bounds__(NW * 64, 2) void attn_dq_kernel(const Params p) {
   using G = Geo<DP>;
@@ -557,7 +560,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_dq_kernel(const Params p) {
   }
   const Item it = p.items[blockIdx.x / p.kv_heads];
   const int hk = blockIdx.x % p.kv_heads;
-  if (!item_ok(it, p) || it.first >= it.q_len) return;
+  if (!item_ok(it, p) || it.first >= it.q_len || it.slot >= p.n_slots) return;
   const int row = wave * 32 + (lane & 31), tpt = NW * 32 / p.group;
   const int tok = it.first + row / p.group, head = hk * p.group + row % p.group;
   const bool valid = row < tpt * p.group && tok < it.q_len;
@@ -581,7 +584,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_dq_kernel(const Params p) {
   }
   delta += other_half(delta);
   const float lse2 = p.lse[t_ * p.heads + h_] * LOG2E - T::LIFT;
-  if (valid && lane < 32) p.delta[t_ * p.heads + h_] = delta;
+  if (valid && lane < 32 && it.begin == 0) p.delta[t_ * p.heads + h_] = delta;                         // (the first of a split walk)
 
   f32x16 acc[DP / 32];
 #pragma unroll
@@ -644,8 +647,17 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_dq_kernel(const Params p) {
       }
     }
   }
-  if (!valid) return;
   const float f = p.scale * (1.f / (1 << T::LIFT));
+  if (it.slot >= 0) {
+    float* out = p.part + (((long)it.slot * p.kv_heads + hk) * (NW * 32) + row) * DP;
+#pragma unroll
+    for (int mb = 0; mb < DP / 32; ++mb)
+#pragma unroll
+      for (int i4 = 0; i4 < 4; ++i4)
+        *reinterpret_cast<f32x4*>(out + mb * 32 + 8 * i4 + 4 * (lane >> 5)) = f32x4{acc[mb][4 * i4] * f, acc[mb][4 * i4 + 1] * f, acc[mb][4 * i4 + 2] * f, acc[mb][4 * i4 + 3] * f};
+    return;
+  }
+  if (!valid) return;
   char* op = const_cast<char*>(p.dq.p) + t_ * p.dq.st + h_ * p.dq.sh;
 #pragma unroll
   for (int mb = 0; mb < DP / 32; ++mb)
@@ -657,6 +669,19 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_dq_kernel(const Params p) {
       v.y = T::pack(acc[mb][4 * i4 + 2] * f, acc[mb][4 * i4 + 3] * f);
       if (d < p.dim) *reinterpret_cast<u32x2*>(op + d * 2) = v;
     }
+}
+
+// adds the parts of split rows: items {q_start, q_len, -, -, first, first slot, slots, -}; a thread adds 4 channels of one row
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void attn_dq_join_kernel(const Params p) {
+  const Item it = p.items[blockIdx.y / p.kv_heads];
+  const int hk = blockIdx.y % p.kv_heads;
+  const int at = blockIdx.x * 256 + threadIdx.x, row = at / (DP / 4), d = at % (DP / 4) * 4;
+  const int tok = it.first + row / p.group, head = hk * p.group + row % p.group;
+  if (row >= 128 / p.group * p.group || tok >= it.q_len || d >= p.dim || !item_ok(it, p) || (long)it.begin + it.end > p.n_slots) return;
+  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < it.end; ++i) sum += *reinterpret_cast<const f32x4*>(p.part + (((long)(it.begin + i) * p.kv_heads + hk) * 128 + row) * DP + d);
+  *reinterpret_cast<u32x2*>(const_cast<char*>(p.dq.p) + (long)(it.q_start + tok) * p.dq.st + (long)head * p.dq.sh + d * 2) = u32x2{T::pack(sum.x, sum.y), T::pack(sum.z, sum.w)};
 }
 
 // dK, dV: one workgroup holds 64 keys of one key head (128 where head_dim > 64), 32 a wave, and walks over the rows (tokens x group) that see
@@ -932,6 +957,7 @@ template <typename T, int DP> int run_fwd(Params p, const dh_attn_info& info, co
 }
 template <typename T, int DP> int run_bwd(Params p, const dh_attn_info& info, const Item* items, hipStream_t st) {
   p.items = items + info.n_fwd + info.n_join;
+  p.n_slots = info.n_dq_slots;
   p.blocks = (int)(info.n_dq * info.kv_heads);
   unsigned more = clear_blocks(p.q_rows - p.clear_q, p.heads, p.dim);
   if (p.blocks + more) {
@@ -939,6 +965,12 @@ template <typename T, int DP> int run_bwd(Params p, const dh_attn_info& info, co
     DH_LAUNCH_CHECK();
   }
   p.items += info.n_dq;
+  if (info.n_dq_join) {
+    hipLaunchKernelGGL((attn_dq_join_kernel<T, DP>), dim3(128 * DP / 4 / 256, (unsigned)(info.n_dq_join * info.kv_heads)), dim3(256), 0, st, p);
+    DH_LAUNCH_CHECK();
+  }
+  p.items += info.n_dq_join;
+  p.n_slots = info.n_dkv_slots;
   p.blocks = (int)(info.n_dkv * info.kv_heads);
   more = clear_blocks(p.k_rows - p.clear_k, p.kv_heads, p.dim);
   if (p.blocks + more) {
@@ -955,9 +987,14 @@ template <typename T, int DP> int run_bwd(Params p, const dh_attn_info& info, co
 }
 
 bool info_ok(const dh_attn_info* i) {
-  return i && heads_ok(i->heads, i->kv_heads, i->head_dim) && i->causal_block >= 0 && i->causal_block <= MAX_ROWS && (i->waves == 1 || i->waves == 4) &&
-         i->ints == 8 * (i->n_fwd + i->n_join + i->n_dq + i->n_dkv + i->n_dkv_join) && i->n_fwd >= 0 && i->n_join >= 0 && i->n_dq >= 0 && i->n_dkv >= 0 && i->n_dkv_join >= 0 && i->n_slots >= 0 && i->n_dkv_slots >= 0 && i->q_rows >= 0 && i->k_rows >= 0 && i->q_rows <= MAX_ROWS && i->k_rows <= MAX_ROWS &&
-         i->n_fwd * i->kv_heads <= INT_MAX - 1024 && i->n_join * i->kv_heads <= 65535 && i->n_dq * i->kv_heads <= INT_MAX - 1024 && i->n_dkv * i->kv_heads <= INT_MAX - 1024 && i->n_dkv_join * i->kv_heads <= 65535;
+  if (!i || !heads_ok(i->heads, i->kv_heads, i->head_dim) || i->causal_block < 0 || i->causal_block > MAX_ROWS || (i->waves != 1 && i->waves != 4)) return false;
+  const int64_t items[3] = {i->n_fwd, i->n_dq, i->n_dkv}, joins[3] = {i->n_join, i->n_dq_join, i->n_dkv_join}, slots[3] = {i->n_slots, i->n_dq_slots, i->n_dkv_slots};
+  int64_t n = 0;
+  for (int k = 0; k < 3; ++k) {
+    if (items[k] < 0 || items[k] > INT_MAX / 8 || items[k] * i->kv_heads > INT_MAX - 1024 || joins[k] < 0 || joins[k] * i->kv_heads > 65535 || slots[k] < 0 || slots[k] > items[k]) return false;
+    n += items[k] + joins[k];
+  }
+  return i->ints == 8 * n && i->q_rows >= 0 && i->k_rows >= 0 && i->q_rows <= MAX_ROWS && i->k_rows <= MAX_ROWS;
 }
 
 }  // namespace
@@ -985,23 +1022,31 @@ extern "C" int dh_attn_plan(const int64_t* q_len, const int64_t* k_len, const in
   // 24 tiles (some 20 us) of a workgroup's walk: a split row's sums go through memory once more, and the join is a launch of its own (packed clips,
   // 64 channels: 87 us with 8, 85 with 24).  Lone waves are split for any saving: long walks meet short ones there, and a join is needed anyway (32
   // queries over 1 .. 32400 keys: 82 us; 87 if it had to save 4 tiles, 130 if 24).
-  const int dp = pad_dim(head_dim), slots_on_chip = 256 * (waves == 1 ? (dp == 128 ? 3 : 6) : dp == 128 ? 2 : 3);       // LDS or registers hold no more
-  const int64_t* ql = q_len; const int64_t* kl = k_len;
-  auto each_tile = [&](auto&& f) {
-    for (int64_t i = 0; i < n_seqs; ++i)
-      for (long t = 0; t < ql[i]; t += tpt) f((keys_seen((int)std::min<long>(ql[i], t + tpt) - 1, (int)ql[i], (int)kl[i], block) + BN - 1) / BN);
+  const int dp = pad_dim(head_dim);
+  struct Share {
+    long piece, save;
+    long pieces(long nt) const { return nt > piece + piece / 8 + save ? (nt + piece - 1) / piece : 1; }
   };
-  long tiles = 0, walks = 0;
-  each_tile([&](long nt) { tiles += nt * kv_heads; walks += kv_heads; });
-  long piece = std::max<long>(4, (tiles + slots_on_chip - 1) / slots_on_chip);
-  auto pieces_of = [&](long nt) -> long { return nt > piece + piece / 8 + (waves == 1 ? 0 : 24) ? (nt + piece - 1) / piece : 1; };
-  if (walks < slots_on_chip)                     // rounding up must not leave a few items for a second round
-    for (;;) {
-      long n = 0, longest = 0;
-      each_tile([&](long nt) { n += pieces_of(nt) * kv_heads; longest = std::max(longest, nt); });
-      if (n <= slots_on_chip || longest <= piece) break;
-      piece += std::max<long>(1, piece / 16);
-    }
+  const int64_t* ql = q_len; const int64_t* kl = k_len;
+  auto share_of = [&](int step, long places, long save) {      // walks of `step` tokens each; places: workgroups that LDS or registers leave room for
+    auto each_walk = [&](auto&& f) {
+      for (int64_t i = 0; i < n_seqs; ++i)
+        for (long t = 0; t < ql[i]; t += step) f((keys_seen((int)std::min<long>(ql[i], t + step) - 1, (int)ql[i], (int)kl[i], block) + BN - 1) / BN);
+    };
+    long tiles = 0, walks = 0;
+    each_walk([&](long nt) { tiles += nt * kv_heads; walks += kv_heads; });
+    Share s{std::max<long>(4, (tiles + places - 1) / places), save};
+    if (walks < places)                          // rounding up must not leave a few items for a second round
+      for (;;) {
+        long n = 0, longest = 0;
+        each_walk([&](long nt) { n += s.pieces(nt) * kv_heads; longest = std::max(longest, nt); });
+        if (n <= places || longest <= s.piece) break;
+        s.piece += std::max<long>(1, s.piece / 16);
+      }
+    return s;
+  };
+  const Share share = share_of(tpt, 256 * (waves == 1 ? (dp == 128 ? 3 : 6) : dp == 128 ? 2 : 3), waves == 1 ? 0 : 24);
+  const Share share_q = share_of(tpt_q, 256 * (dp == 128 ? 2 : 3), 24);      // dQ: the forward's walk, always in tiles of 128 rows
   // The same for the rows of dK and dV.  A split key tile costs a trip of its 32-bit sums through memory, so pieces are 24 tiles of 64 rows at
   // least.  One share a place where three workgroups fit a CU; four where one does (training window, 128 channels: 3.20, 3.09, 3.04 ms with two,
   // one, four shares of 256; packed clips, 64 channels: 124, 121 us with two, one share of 768).
@@ -1017,67 +1062,58 @@ extern "C" int dh_attn_plan(const int64_t* q_len, const int64_t* k_len, const in
   Item* base = reinterpret_cast<Item*>(plan);
   const long cap = plan ? plan_ints / 8 : 0;
   Writer w{base, cap, 0};
-  long slots = 0, slots_k = 0;
-  int64_t counts[5];
-  for (int pass = 0; pass < 5; ++pass) {         // forward items, joins, dQ items, dK / dV items, joins
+  int64_t counts[6], slots[6];
+  for (int pass = 0; pass < 6; ++pass) {         // forward items and joins, dQ items and joins, dK / dV items and joins
     const long from = w.n;
     long qs = 0, ka = 0, slot = 0;
+    // a walk of nt tiles in n pieces: an item each (piece x: from tile a on, to tile b), or what joins them
+    auto put = [&](Item it, long nt, long n, auto&& range) {
+      if (pass % 2 == 0) {
+        if (n == 1) w.put(it);
+        else
+          for (long x = 0; x < n; ++x) {
+            range(it, nt * x / n, nt * (x + 1) / n);
+            it.slot = (int)slot++;
+            w.put(it);
+          }
+      } else if (n > 1) {
+        it.begin = (int)slot;
+        it.end = (int)n;
+        slot += n;
+        w.put(it);
+      }
+    };
     for (int64_t i = 0; i < n_seqs; ++i) {
       const int m = (int)q_len[i], n = (int)k_len[i];
       const int ks = (int)(k_start ? k_start[i] : ka);
-      if (pass < 3) {
-        const int step = pass == 2 ? tpt_q : tpt;
+      if (pass < 4) {
+        const int step = pass < 2 ? tpt : tpt_q;
         for (int t = 0; t < m; t += step) {
           const int e = keys_seen(std::min(m, t + step) - 1, m, n, block);
-          Item it{(int)qs, m, ks, n, t, 0, e, -1};
           const long nt = (e + BN - 1) / BN;
-          const long pieces = pieces_of(nt);
-          if (pass == 2 || (pass == 0 && pieces == 1)) w.put(it);
-          else if (pass == 0) {
-            for (long x = 0; x < pieces; ++x) {
-              it.begin = (int)(nt * x / pieces * BN);
-              it.end = (int)std::min<long>(e, nt * (x + 1) / pieces * BN);
-              it.slot = (int)slot++;
-              w.put(it);
-            }
-          } else if (pieces > 1) {
-            it.begin = (int)slot;
-            it.end = (int)pieces;
-            slot += pieces;
-            w.put(it);
-          }
+          put(Item{(int)qs, m, ks, n, t, 0, e, -1}, nt, (pass < 2 ? share : share_q).pieces(nt), [&](Item& it, long a, long b) {
+            it.begin = (int)(a * BN);
+            it.end = (int)std::min<long>(e, b * BN);
+          });
         }
       } else {
         for (int x = 0; x < n; x += dkv_keys) {
           const int t0 = (int)rows_of(i, x);
-          Item it{(int)qs, m, ks, n, x, t0, m, -1};
           const long nt = ((long)m - t0 + tpt_k - 1) / tpt_k;
-          const long pieces = nt > piece_k + piece_k / 4 ? (nt + piece_k - 1) / piece_k : 1;
-          if (pass == 3 && pieces == 1) w.put(it);
-          else if (pass == 3) {
-            for (long y = 0; y < pieces; ++y) {
-              it.begin = (int)(t0 + nt * y / pieces * tpt_k);
-              it.end = (int)std::min<long>(m, t0 + nt * (y + 1) / pieces * tpt_k);
-              it.slot = (int)slot++;
-              w.put(it);
-            }
-          } else if (pieces > 1) {
-            it.begin = (int)slot;
-            it.end = (int)pieces;
-            slot += pieces;
-            w.put(it);
-          }
+          put(Item{(int)qs, m, ks, n, x, t0, m, -1}, nt, nt > piece_k + piece_k / 4 ? (nt + piece_k - 1) / piece_k : 1, [&](Item& it, long a, long b) {
+            it.begin = (int)(t0 + a * tpt_k);
+            it.end = (int)std::min<long>(m, t0 + b * tpt_k);
+          });
         }
       }
       qs += m;
       ka += n;
       if (slot > INT_MAX || w.n > INT_MAX / 8) return DH_ERR_ARG;
     }
-    if (pass == 0) slots = slot;
-    if (pass == 3) slots_k = slot;
+    slots[pass] = slot;
     counts[pass] = w.n - from;
     // longest first, so that the last workgroups to start are short ones
-    if (pass != 1 && pass != 4 && base && w.n <= cap) std::sort(base + from, base + w.n, longer);
+    if (pass % 2 == 0 && base && w.n <= cap) std::sort(base + from, base + w.n, longer);
   }
   // key ranges of two sequences that share rows: fine to read, but their gradients would be written twice
   bool shared = false;
@@ -1095,8 +1131,9 @@ extern "C" int dh_attn_plan(const int64_t* q_len, const int64_t* k_len, const in
   info->ints = w.n * 8;
   info->heads = heads; info->kv_heads = kv_heads; info->head_dim = head_dim; info->causal_block = block;
   info->waves = waves;
-  info->n_fwd = counts[0]; info->n_join = counts[1]; info->n_dq = counts[2]; info->n_dkv = counts[3]; info->n_dkv_join = counts[4];
-  info->n_slots = slots; info->n_dkv_slots = slots_k; info->q_rows = q_rows; info->k_rows = k_rows; info->keys_shared = shared; info->k_total = k_at;
+  info->n_fwd = counts[0]; info->n_join = counts[1]; info->n_dq = counts[2]; info->n_dq_join = counts[3]; info->n_dkv = counts[4];
+  info->n_dkv_join = counts[5];
+  info->n_slots = slots[0]; info->n_dq_slots = slots[2]; info->n_dkv_slots = slots[4]; info->q_rows = q_rows; info->k_rows = k_rows; info->keys_shared = shared; info->k_total = k_at;
   if (!info_ok(info)) return DH_ERR_ARG;
   if (plan && plan_ints < info->ints) return DH_ERR_WORKSPACE;
   return DH_OK;
@@ -1133,7 +1170,9 @@ extern "C" int dh_attn_fwd(const void* q, int64_t q_st, int64_t q_sh, const void
 static size_t delta_floats(const dh_attn_info* i) { return ((size_t)i->q_rows * i->heads + 3) / 4 * 4; }
 extern "C" size_t dh_attn_bwd_workspace_bytes(const dh_attn_info* info) {
   if (!info_ok(info)) return 0;
-  return (delta_floats(info) + (size_t)info->n_dkv_slots * info->kv_heads * (pad_dim((int)info->head_dim) == 128 ? Dkv<128>::KEYS : Dkv<64>::KEYS) * 2 * pad_dim((int)info->head_dim)) * sizeof(float);
+  // the parts of dQ are joined before those of dK and dV are written
+  const size_t dp = pad_dim((int)info->head_dim), keys = dp == 128 ? Dkv<128>::KEYS : Dkv<64>::KEYS;
+  return (delta_floats(info) + std::max((size_t)info->n_dq_slots * 128, (size_t)info->n_dkv_slots * keys * 2) * info->kv_heads * dp) * sizeof(float);
 }
 
 extern "C" int dh_attn_bwd(const void* grad, int64_t g_st, int64_t g_sh, const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh,
@@ -1160,7 +1199,7 @@ extern "C" int dh_attn_bwd(const void* grad, int64_t g_st, int64_t g_sh, const v
   if (rest_k && (!view_ok(p.dk, k_rows, info->kv_heads, dim) || !view_ok(p.dv, k_rows, info->kv_heads, dim))) return DH_ERR_ARG;
   if (info->n_dkv && (!view_ok(p.k, k_rows, info->kv_heads, dim, true) || !view_ok(p.v, k_rows, info->kv_heads, dim, true) || !view_ok(p.dk, k_rows, info->kv_heads, dim) ||
                       !view_ok(p.dv, k_rows, info->kv_heads, dim))) return DH_ERR_ARG;
-  p.low = (char*)const_cast<void*>(o_low); p.lse = const_cast<float*>(lse); p.delta = (float*)workspace; p.part = (float*)workspace + delta_floats(info); p.n_slots = info->n_dkv_slots;
+  p.low = (char*)const_cast<void*>(o_low); p.lse = const_cast<float*>(lse); p.delta = (float*)workspace; p.part = (float*)workspace + delta_floats(info);
   p.kv_heads = (int)info->kv_heads; p.heads = (int)info->heads; p.group = p.heads / p.kv_heads; p.dim = dim; p.block = (int)info->causal_block;
   p.q_rows = (int)q_rows; p.k_rows = (int)k_rows; p.clear_q = clear_rest ? (int)info->q_rows : p.q_rows; p.clear_k = clear_rest ? (int)info->k_rows : p.k_rows; p.scale = scale; p.c = scale * LOG2E;
   const Item* items = reinterpret_cast<const Item*>(plan);

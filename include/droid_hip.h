@@ -484,7 +484,7 @@ int dh_reproject_ex(const float* poses, const float* disps, const float* intrins
  *   o = softmax(scale q k^T) v (scale > 0), lse [q_rows, heads] f32 = natural logarithm of the row's sum.
  * Rows behind the last sequence (of o, lse, dq) and behind the last key (of dk, dv) are left as they were, or cleared where clear_rest
  * (o, gradients 0, lse -inf).  Rows of dk, dv between the sequences' keys (k_start with gaps) are left as they were.
- * Values are expected to be finite where a gradient is wanted.  A non-finite value (q, k or v) reaches the rows that see it and no others.
+ * Scores (scale q.k) up to 10^8 in size.  Values are expected to be finite where a gradient is wanted.  A non-finite value (q, k or v) reaches the rows that see it and no others.
  *
  * dh_attn_plan runs on the HOST: it lays out the work items of one set of lengths.  plan_host NULL: only fills *info (info->ints = ints
  * wanted); else writes plan_host[0 .. info->ints).  The caller copies it to the device and passes it, with *info, to every call on these
@@ -497,8 +497,8 @@ typedef struct {
   int64_t ints;                                         /* length of the plan */
   int64_t heads, kv_heads, head_dim, causal_block;
   int64_t waves;                                        /* wavefronts (32 rows each) of a forward workgroup */
-  int64_t n_fwd, n_join, n_dq, n_dkv, n_dkv_join;       /* work items */
-  int64_t n_slots, n_dkv_slots;                         /* partial results of split rows / keys, in the workspaces */
+  int64_t n_fwd, n_join, n_dq, n_dq_join, n_dkv, n_dkv_join;                 /* work items */
+  int64_t n_slots, n_dq_slots, n_dkv_slots;                         /* partial results of split rows / keys, in the workspaces */
   int64_t q_rows, k_rows;                               /* rows that q and k must have at least */
   int64_t k_total;                                      /* sum of k_len */
   int64_t keys_shared;                                  /* two sequences share keys: no backward */

@@ -16,14 +16,15 @@ import droid_backends as db  # noqa: E402
 from droid_amd import attention as at  # noqa: E402
 from oracle import attention as oa  # noqa: E402
 
-FIELDS = ["ints", "heads", "kv_heads", "head_dim", "causal_block", "waves", "n_fwd", "n_join", "n_dq", "n_dkv", "n_dkv_join", "n_slots", "n_dkv_slots", "q_rows", "k_rows", "k_total", "keys_shared"]
+FIELDS = ["ints", "heads", "kv_heads", "head_dim", "causal_block", "waves", "n_fwd", "n_join", "n_dq", "n_dq_join", "n_dkv", "n_dkv_join", "n_slots", "n_dq_slots", "n_dkv_slots",
+          "q_rows", "k_rows", "k_total", "keys_shared"]
 
 
 def plan(lengths, heads, kv_heads, dim, **kw):
     p = at.PackedPlan(lengths, heads, kv_heads, dim, device="cpu", **kw)
     info = dict(zip(FIELDS, p.info.tolist()))
     items = p.items.view(-1, 8).tolist()
-    cut = list(itertools.accumulate([0] + [info[n] for n in ("n_fwd", "n_join", "n_dq", "n_dkv", "n_dkv_join")]))
+    cut = list(itertools.accumulate([0] + [info[n] for n in ("n_fwd", "n_join", "n_dq", "n_dq_join", "n_dkv", "n_dkv_join")]))
     return info, [items[a:b] for a, b in zip(cut, cut[1:])]
 
 
@@ -36,7 +37,7 @@ PLANS = [([1], None, 1, 1, 0), ([48], None, 4, 4, 0), ([5, 0, 300, 1], None, 8, 
 def test_plan_covers_every_row_and_key_once(lengths, key_lengths, heads, kv_heads, block, dim, keys_a_tile):
     """each visible (row, key) pair is in exactly one forward item, one dQ item and one dK / dV item"""
     keys = lengths if key_lengths is None else key_lengths
-    info, (fwd, join, dq, dkv, dkv_join) = plan(lengths, heads, kv_heads, dim, key_lengths=key_lengths, causal_block=block)
+    info, (fwd, join, dq, dq_join, dkv, dkv_join) = plan(lengths, heads, kv_heads, dim, key_lengths=key_lengths, causal_block=block)
     assert info["q_rows"] == sum(lengths) and info["k_rows"] == sum(keys) == info["k_total"] and not info["keys_shared"]
     group = heads // kv_heads
     q0 = k0 = 0
@@ -58,10 +59,9 @@ def test_plan_covers_every_row_and_key_once(lengths, key_lengths, heads, kv_head
                 hit[begin:end, first:first + keys_a_tile] += 1
         assert bool((hit[seen] == 1).all()) and bool((hit <= 1).all())
         q0, k0 = q0 + m, k0 + l
-    slots = sorted(x for j in join for x in range(j[5], j[5] + j[6]))
-    assert slots == list(range(info["n_slots"])) == sorted(i[7] for i in fwd if i[7] >= 0)
-    slots = sorted(x for j in dkv_join for x in range(j[5], j[5] + j[6]))
-    assert slots == list(range(info["n_dkv_slots"])) == sorted(i[7] for i in dkv if i[7] >= 0)
+    for items, joins, n in ((fwd, join, "n_slots"), (dq, dq_join, "n_dq_slots"), (dkv, dkv_join, "n_dkv_slots")):
+        slots = sorted(x for j in joins for x in range(j[5], j[5] + j[6]))
+        assert slots == list(range(info[n])) == sorted(i[7] for i in items if i[7] >= 0)
 
 
 def test_plan_of_shared_keys_and_gaps():
@@ -105,7 +105,7 @@ def test_c_entries_refuse_before_a_launch():
         buf = None if room is None else (ctypes.c_int32 * max(1, room))()
         return lib.dh_attn_plan(arr(lengths), arr(keys), arr(starts), i64(len(lengths)), heads, kv, dim, i64(block), buf, i64(room or 0), info)
 
-    assert make([5], [9]) == 0 and info[0] == 8 * sum(info[6:11])
+    assert make([5], [9]) == 0 and info[0] == 8 * sum(info[6:12])
     assert make([5], [9], room=info[0] - 1) == 2                             # too small a buffer: nothing is written behind it
     assert make([5], [9], room=int(info[0])) == 0
     assert make([-1], [9]) == 1 and make([5], [9], starts=[-3]) == 1 and make([5], [9], dim=20) == 1 and make([5], [9], heads=5) == 1 and make([5], [9], block=-1) == 1
@@ -118,7 +118,7 @@ def test_c_entries_refuse_before_a_launch():
     for bad in (dict(q=0), dict(q=8), dict(k=0), dict(v=264), dict(o=0), dict(low=8), dict(lse=0), dict(plan=0), dict(dtype=1), dict(dtype=2), dict(rows=4), dict(keys=8), dict(scale=0.0),
                 dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(st=(252, 64)), dict(st=(-256, 64)), dict(st=(1 << 25, 64)), dict(st=(256, 1 << 26)), dict(info=None)):
         assert fwd(**bad) == 1, bad
-    assert make([1], [100000], heads=8, kv=1) == 0 and info[11] > 0 and lib.dh_attn_fwd_workspace_bytes(info) > 0
+    assert make([1], [100000], heads=8, kv=1) == 0 and info[12] > 0 and lib.dh_attn_fwd_workspace_bytes(info) > 0
     assert fwd(rows=1, keys=100000) == 2                                     # split rows need the workspace
 
     def bwd(ws=256, wsb=1 << 20, dtype=0, rows=5, keys=9, dq=256, dk=256, plan=256, lse=256):

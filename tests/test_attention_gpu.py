@@ -66,7 +66,7 @@ def test_few_queries_over_long_keys(dtype, heads, kv_heads, dim, block):
     lengths, keys = [1, 1, 2, 1, 1, 1], [1, 5000, 2047, 0, 64, 12345]
     q, k, v, g = inputs(lengths, keys, heads, kv_heads, dim, dtype, 5)
     plan = at.PackedPlan(lengths, heads, kv_heads, dim, key_lengths=keys, causal_block=block)
-    assert int(plan.info[7]) > 0                                             # (split rows)
+    assert int(plan.info[7]) > 0 and int(plan.info[9]) > 0                   # (rows split in the forward and in the backward)
     r = oa.attention(q, k, v, lengths, keys, block=block, grad=g)
     o, lse = at.packed_attention(q, k, v, plan, return_lse=True)
     near(o, r["o"], r["o_err"], "o")
@@ -206,13 +206,27 @@ def test_many_rows_over_few_keys(dtype, heads, kv_heads, dim, lengths, keys, blo
     """gradients of keys that are split over their rows and joined"""
     q, k, v, g = inputs(lengths, keys, heads, kv_heads, dim, dtype, 6)
     plan = at.PackedPlan(lengths, heads, kv_heads, dim, key_lengths=keys, causal_block=block)
-    assert int(plan.info[10]) > 0
+    assert int(plan.info[11]) > 0                                            # (split keys)
     r = oa.attention(q, k, v, lengths, keys, block=block, grad=g)
     leaves = [t.clone().requires_grad_() for t in (q, k, v)]
     o = at.packed_attention(*leaves, plan)
     near(o, r["o"], r["o_err"], "o")
     for n, t in zip(("dq", "dk", "dv"), torch.autograd.grad(o, leaves, g)):
         near(t, r[n], r[n + "_err"], n)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_scores_as_large_as_they_may_be(sign, dtype):
+    """scores of 2.5 10^7 and 5 10^7, of either sign, far apart: one key's weight is one"""
+    q = torch.full((3, 2, 64), 2048.0, dtype=dtype, device="cuda")
+    k = torch.full((3, 1, 64), sign * 1536.0, dtype=dtype, device="cuda")
+    k[1] *= 2 if sign > 0 else 0.5                                           # the second key wins wherever it is seen
+    v = rand((3, 1, 64), dtype, 1)
+    o, lse = at.packed_attention(q, k, v, at.PackedPlan([3], 2, 1, 64, causal_block=1), return_lse=True)
+    for i, winner in enumerate((0, 1, 1)):
+        assert torch.equal(o[i], v[winner].expand(2, -1)), i
+    assert bool(torch.isfinite(lse).all())
 
 
 def test_attention_gradient_against_differences():
