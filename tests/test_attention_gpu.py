@@ -385,6 +385,54 @@ def test_offsets_beyond_32_bits():
     near(y[0], rq["y"], rq["y_err"], "rotation")
 
 
+def test_raw_c_abi_on_a_side_stream():
+    """the C entries with plain pointers on a stream of the caller's: the binding's bits, rows behind the sequences left as they were"""
+    import ctypes
+    from tests.test_attention_cpu import FIELDS
+    lib = ctypes.CDLL(os.path.join(os.path.dirname(at.droid_backends.__file__), "libdroid_hip.so"))
+    i64, ptr, f32 = ctypes.c_int64, ctypes.c_void_p, ctypes.c_float
+    for name in ("dh_attn_fwd_workspace_bytes", "dh_attn_bwd_workspace_bytes", "dh_qk_norm_rope_bwd_workspace_bytes"):
+        getattr(lib, name).restype = ctypes.c_size_t
+    lengths, keys, h, kv, d, pad = [1, 4, 2], [9000, 30, 5000], 4, 2, 64, 3
+    q, k, v, g = inputs(lengths, keys, h, kv, d, F16, 70, pad)
+    plan = at.PackedPlan(lengths, h, kv, d, key_lengths=keys, causal_block=1)
+    o, lse, low = at.droid_backends.attention_forward(q, k, v, plan.items, plan.info, 0.125, None, True)
+    want = [o, lse] + at.droid_backends.attention_backward(g, q, k, v, o, lse, low, plan.items, plan.info, 0.125)
+    info = (i64 * len(FIELDS))()
+    ql, kl = (i64 * 3)(*lengths), (i64 * 3)(*keys)
+    assert lib.dh_attn_plan(ql, kl, None, i64(3), h, kv, d, i64(1), None, i64(0), info) == 0
+    items = (ctypes.c_int32 * info[0])()
+    assert lib.dh_attn_plan(ql, kl, None, i64(3), h, kv, d, i64(1), items, i64(info[0]), info) == 0
+    items = torch.frombuffer(items, dtype=torch.int32).clone().cuda()
+    o2, lse2, dq, dk, dv = [torch.full_like(t, 7.0) for t in want]
+    low2 = torch.empty_like(o2)
+    wf, wb = lib.dh_attn_fwd_workspace_bytes(info), lib.dh_attn_bwd_workspace_bytes(info)
+    ws = torch.empty(max(wf, wb) + 16, dtype=torch.uint8, device="cuda")
+    t = lambda x: (ptr(x.data_ptr()), i64(x.stride(0)), i64(x.stride(1)))  # noqa: E731
+    p = lambda x: ptr(x.data_ptr())  # noqa: E731
+    torch.cuda.synchronize()
+    st = torch.cuda.Stream()
+    tail = (p(items), info, 0, i64(q.shape[0]), i64(k.shape[0]), f32(0.125), 0, p(ws))
+    assert lib.dh_attn_fwd(*t(q), *t(k), *t(v), *t(o2), p(low2), p(lse2), *tail, ctypes.c_size_t(wf), ptr(st.cuda_stream)) == 0
+    assert lib.dh_attn_bwd(*t(g), *t(q), *t(k), *t(v), *t(o2), p(low2), p(lse2), *t(dq), *t(dk), *t(dv), *tail, ctypes.c_size_t(wb), ptr(st.cuda_stream)) == 0
+    st.synchronize()
+    for a, b, n in zip((o2, lse2, dq, dk, dv), want, (sum(lengths),) * 3 + (sum(keys),) * 2):
+        assert torch.equal(a[:n], b[:n]) and bool((a[n:] == 7).all())
+    pos, fr, w, sec = torch.arange(len(q)).int().cuda(), torch.rand(32).cuda(), torch.rand(d).cuda(), (ctypes.c_int * 4)(32, 0, 0, 0)
+    kk = k[:len(q)]
+    want = list(at.qk_norm_rope(q, kk, pos, fr, [32], w, w)) + at.droid_backends.qk_norm_rope_backward(g, kk, q, kk, pos, fr, [32], w, w, True, 1e-6, False)
+    got = [torch.empty_like(x) for x in want]
+    tail = (p(pos), 0, p(fr), sec, 1, p(w), p(w), 1, 0, i64(len(q)), h, kv, d, 1, f32(1e-6), 0)
+    torch.cuda.synchronize()
+    assert lib.dh_qk_norm_rope_fwd(*t(q), *t(kk), *t(got[0]), *t(got[1]), *tail, ptr(st.cuda_stream)) == 0
+    n = lib.dh_qk_norm_rope_bwd_workspace_bytes(d)
+    ws = torch.empty(n, dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    assert lib.dh_qk_norm_rope_bwd(*t(g), *t(kk), *t(q), *t(kk), *t(got[2]), *t(got[3]), p(got[4]), p(got[5]), *tail, p(ws), ctypes.c_size_t(n), ptr(st.cuda_stream)) == 0
+    st.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_attention_refusals():
     plan = at.PackedPlan([8], 4, 2, 64)
     q, k, v, g = inputs([8], None, 4, 2, 64, F16)
