@@ -1014,7 +1014,8 @@ extern "C" int dh_attn_plan(const int64_t* q_len, const int64_t* k_len, const in
     most = std::max<long>(most, q_len[i]);
     if (q_rows > MAX_ROWS || k_rows > MAX_ROWS || k_at > (1l << 40)) return DH_ERR_ARG;
   }
-  // rows a workgroup: one wave where a tile of 32 holds every row of the longest sequence (decoding), else 128
+  // rows a workgroup: one wave where a tile of 32 holds every row of the longest sequence, else 128 (32 single queries of 16/2 heads: 82 us against
+  // 109 with 128 rows; 768 queries of 8 heads over 23040 keys: 90 us against 59 with 128)
   const int waves = most * group <= 32 ? 1 : 4;
   const int tpt = waves * 32 / group, tpt_q = 128 / group;
   // Long walks over the keys become several work items (pieces of whole key tiles, joined afterwards) where they would outlast the rest:

@@ -3,7 +3,8 @@
 //   z = x r w,  r = 1 / sqrt(mean(x^2) + eps);   pair (a, b) of z -> (a cos t - b sin t, a sin t + b cos t),  t = position[axis(pair)] inv_freq[pair]
 //   dz = rotation by -t of dy;  dw = sum over tokens and heads of dz x r;  dx = r w dz - x r^3 mean(w dz x)
 //
-// Bound by memory: each head is read once and written once (backward: x and dy read, dx written).  A row (one head of one token) belongs to
+// Bound by memory: each head is read once and written once (backward: x and dy read, dx written): 30000 tokens x 20 heads of 128 (bf16) take
+// 73 us forward = 4.2 TB/s and 119 us backward = 3.9 TB/s, where a large copy reaches 4.6.  A row (one head of one token) belongs to
 // dim / (2 V) neighbouring lanes; a lane holds V channels and their V partners, so a rotation stays inside a lane, and the sums over a head
 // are a few exchanges between neighbours.  The angles belong to the token: a lane computes its sines and cosines once and keeps them for
 // all heads of its token.
@@ -348,7 +349,8 @@ template <typename Io, int V, bool ADJ, bool NORM> int launch(RopeParams& p, boo
   while ((1 << p.shift) < lanes) ++p.shift;
   const int slots = 64 >> p.shift, total = p.heads[0] + p.heads[1];
   const long groups = (p.tokens + 4 * slots - 1) / (4 * slots);
-  // few tokens: the heads are spread over workgroups as well, until every place on the chip has a workgroup
+  // few tokens: the heads are spread over workgroups as well, until every place on the chip has one: four a CU forward, two backward (5376 tokens x
+  // 16 heads of 64: forward 10.2 us, with two 11.0, with eight 14.4; backward 21 us, with four 32)
   const int parts = (int)std::min<long>(total, std::max<long>(1, (bwd ? 512 : 1024) / groups));
   p.chunk = (total + parts - 1) / parts;
   const int gy = (total + p.chunk - 1) / p.chunk;
@@ -371,7 +373,8 @@ template <typename Io, int V> int pick(RopeParams& p, bool adjacent, bool norm, 
   return DH_ERR_UNSUPPORTED;
 }
 template <typename Io> int pick_v(RopeParams& p, bool adjacent, bool norm, bool bwd, int* blocks, hipStream_t st) {
-  // the backward holds x, dy and the sums of dw: with 8 channels and their partners a lane it needs over 256 registers, one wave a SIMD
+  // the backward holds x, dy and the sums of dw: with 8 channels and their partners a lane it needs over 256 registers, one wave a SIMD (30000
+  // tokens x 20 heads of 128: 177 us against 134 with 4 channels)
   const int v = std::min(bwd ? 4 : 8, vector_of(p, adjacent, Io::SIZE, bwd));
   return v == 8 ? pick<Io, 8>(p, adjacent, norm, bwd, blocks, st) : v == 4 ? pick<Io, 4>(p, adjacent, norm, bwd, blocks, st)
        : v == 2 ? pick<Io, 2>(p, adjacent, norm, bwd, blocks, st) : pick<Io, 1>(p, adjacent, norm, bwd, blocks, st);
