@@ -385,6 +385,45 @@ def test_offsets_beyond_32_bits():
     near(y[0], rq["y"], rq["y_err"], "rotation")
 
 
+def test_nothing_on_one_side():
+    """keys without queries get zero gradients, queries without keys zero results and gradients; the same tensor may be all three inputs"""
+    q, k, v, g = inputs([0, 6], [5, 0], 4, 2, 64, BF16)
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    o, lse = at.packed_attention(*leaves, at.PackedPlan([0, 6], 4, 2, 64, key_lengths=[5, 0], causal_block=1), return_lse=True)
+    assert not o.any() and bool((lse == -math.inf).all()) and not lse.requires_grad
+    assert all(not t.any() for t in torch.autograd.grad(o, leaves, g))
+    k, v = rand((300, 2, 64), BF16, 1).requires_grad_(), rand((300, 2, 64), BF16, 2).requires_grad_()
+    q = rand((4, 4, 64), BF16, 3).requires_grad_()                           # no sequence at all has queries
+    o = at.packed_attention(q, k, v, at.PackedPlan([0], 4, 2, 64, key_lengths=[300]))
+    assert not o.any() and all(not t.any() for t in torch.autograd.grad(o, (q, k, v), g[:4]))
+    x = rand((50, 3, 64), F16, 4).requires_grad_()
+    g = rand((50, 3, 64), F16, 5)
+    r = oa.attention(x.detach(), x.detach(), x.detach(), [50], block=1, grad=g)
+    (dx,) = torch.autograd.grad(at.packed_attention(x, x, x, at.PackedPlan([50], 3, 3, 64, causal_block=1)), x, g)
+    u = oa.half_step(F16)
+    near(dx, r["dq"] + r["dk"] + r["dv"], sum(r[n + "_err"] + 2 * u * r[n].abs() for n in ("dq", "dk", "dv")), "dx")
+    a, b = at.qk_norm_rope(x, x[:, :0], torch.arange(50, device="cuda"), torch.ones(32, device="cuda"), [32])
+    assert a.shape == x.shape and b.shape == (50, 0, 64)
+    torch.autograd.grad(a.float().square().sum(), x)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_rows_that_see_nothing_may_hold_anything(d):
+    """NaN queries and gradients in rows whose mask leaves nothing: results and gradients are those of finite rows"""
+    q, k, v, g = inputs([300], [170], 4, 2, d, BF16, 80)
+    plan = at.PackedPlan([300], 4, 2, d, key_lengths=[170], causal_block=1)
+
+    def step(q, g):
+        leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+        o = at.packed_attention(*leaves, plan)
+        return [o] + list(torch.autograd.grad(o, leaves, g))
+
+    want = step(q, g)
+    q[:130], g[:130] = float("nan"), float("nan")
+    got = step(q, g)
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and not got[0][:130].any() and not got[1][:130].any()
+
+
 def test_raw_c_abi_on_a_side_stream():
     """the C entries with plain pointers on a stream of the caller's: the binding's bits, rows behind the sequences left as they were"""
     import ctypes
