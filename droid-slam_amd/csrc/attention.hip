@@ -47,7 +47,7 @@ typedef __attribute__((address_space(3))) char lds_char;
 
 struct F16 {
   using V8 = f16x8;
-  // p ~ 1 / (keys) and dS are lifted by 2^4 before they are rounded: 1 / 262144 is still a normal number, and a |dS| of 4094 still finite
+  // p ~ 1 / (keys) and dS are lifted by 2^4 before they are rounded: 1 / 262144 is still a normal number.  A dS has no bound: see Fit.
   static constexpr int LIFT = 4;
   static constexpr unsigned ONE = 0x3c00, INF = 0x7c00;
   static __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
@@ -546,6 +546,35 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const Params p, int rows
 }
 
 // ------------------------------------------------------------------------------------------------------------ backward
+// fp16 holds numbers up to 65504 where dS may be any size, however small the gradients that it sums to (a loss scale makes such dO).  So the
+// columns of dS^T that a lane's sum is made of (a row's for dQ, a key's for dK) get a power of two of their own when one of them passes 2^15: it is
+// taken out of the sum again at the end.  Until then there is only the largest |dS| to look at (some 10 instructions to 16 scores; training clips, fp16: 169 -> 175 us).
+template <typename T, int N> struct Fit {
+  float factor = 1.f, most = 32768.f;
+  // before s is packed; both halves of the wave hold parts of the same column
+  __device__ __forceinline__ void operator()(f32x16& s, f32x16 (&acc)[N]) {
+    if constexpr (T::LIFT != 0) {
+      float mx = 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, fabsf(s[i]));
+      if (__any(mx > most)) {
+        RARE_BRANCH();
+        mx = fmaxf(mx, other_half(mx));
+        // the largest becomes 2^13 .. 2^14: two more doublings fit before the sums are scaled again
+        const float to = mx * factor > 32768.f ? ldexpf(1.f, 14 - __builtin_amdgcn_frexp_expf(mx)) : factor, a = to / factor;
+        factor = to;
+        most = to < 1.f ? -1.f : 32768.f;                                    // from now on every s is scaled
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] *= to;
+#pragma unroll
+        for (int mb = 0; mb < N; ++mb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) acc[mb][i] *= a;
+      }
+    }
+  }
+};
+
 // dQ: the forward's walk over the keys with dO next to Q.  S^T and dP^T = V dO^T give dS^T in the layout of a B operand; the K tile is
 // read a second time transposed for dQ^T = K^T dS^T.  Writes delta for attn_dkv_kernel on the way.  Split as the forward is; 1.18 PFLOP/s on a
 // training window of 14400 tokens (128 channels).
@@ -591,6 +620,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_dq_kernel(const Params p) {
   for (int mb = 0; mb < DP / 32; ++mb)
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[mb][i] = 0.f;
+  Fit<T, DP / 32> fit;
   TileLoader<DP, NW, BN, true> lk, lv;
   lk.init(p.k, p.dim, 1, BN);
   lv.init(p.v, p.dim, 1, BN);
@@ -637,6 +667,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_dq_kernel(const Params p) {
         for (int i = 0; i < 16; ++i)
           if (b * 32 + 8 * (i / 4) + (i & 3) >= end) s[i] = 0.f;
       }
+      fit(s, acc);
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks) {
         u32x4 df;
@@ -647,7 +678,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_dq_kernel(const Params p) {
       }
     }
   }
-  const float f = p.scale * (1.f / (1 << T::LIFT));
+  const float f = p.scale / fit.factor * (1.f / (1 << T::LIFT));
   if (it.slot >= 0) {
     float* out = p.part + (((long)it.slot * p.kv_heads + hk) * (NW * 32) + row) * DP;
 #pragma unroll
@@ -743,6 +774,7 @@ __global__ __launch_bounds__(Dkv<DP>::WAVES * 64, DP == 128 ? 2 : 3) void attn_d
   for (int mb = 0; mb < DP / 32; ++mb)
 #pragma unroll
     for (int i = 0; i < 16; ++i) dk[mb][i] = dv[mb][i] = 0.f;
+  Fit<T, DP / 32> fit;
 
   const int tpt = DKV_ROWS / p.group;                                        // tokens a tile
   TileLoader<DP, DKV_WAVES, DKV_ROWS, false> lq, lg;
@@ -828,6 +860,7 @@ __global__ __launch_bounds__(Dkv<DP>::WAVES * 64, DP == 128 ? 2 : 3) void attn_d
             if (first_tok + tok[j] < from) s[4 * i4 + j] = dp[4 * i4 + j] = 0.f;
         }
       }
+      fit(dp, dk);
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks) {
         u32x4 pf, df;
@@ -846,6 +879,13 @@ __global__ __launch_bounds__(Dkv<DP>::WAVES * 64, DP == 128 ? 2 : 3) void attn_d
     if (t + 1 < tiles) park(t + 1);                                          // (its buffer was last read before this iteration's barrier)
   }
   if (tiles == 0) DMA_WAIT_BARRIER();                                        // (V is still on its way)
+  if constexpr (T::LIFT != 0) {
+    const float a = 1.f / fit.factor;
+#pragma unroll
+    for (int mb = 0; mb < DP / 32; ++mb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) dk[mb][i] *= a;
+  }
   if constexpr (Dkv<DP>::RW == 2) {                                          // the two halves of the rows meet in LDS, where the tiles were
     float* sum = reinterpret_cast<float*>(dyn) + wave * (DP * 64) + lane;
     __syncthreads();

@@ -1,0 +1,49 @@
+"""Token operators on the GPU at the ends of their range: results against the definition, within bounds that follow from the roundings."""
+import os
+import sys
+
+import pytest
+import torch
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+for p in (ROOT, os.path.join(ROOT, "droid-slam_amd")):
+    if p not in sys.path:
+        sys.path.insert(0, p)
+
+from droid_amd import attention as at  # noqa: E402
+from oracle import attention as oa  # noqa: E402
+from tests.test_attention_gpu import BF16, F16, inputs, near, rand  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("size", [25, 200, 1000])
+def test_gradients_whose_factors_are_larger_than_fp16(d, size):
+    """two keys of equal weight and opposite values under a large gradient: dS = +-d size / 2 is past fp16's numbers (lifted by 2^4 past them even
+    sooner), every gradient is inside them"""
+    q, k, v = torch.zeros(3, 2, d), rand((2, 1, d), F16, 1, 0.25).cpu().float(), torch.ones(2, 1, d)
+    q[..., 1], k[:, :, 1], v[1] = 3.0, 0.5, -1.0                             # equal scores: weights of one half
+    g = torch.full((3, 2, d), float(size)) * torch.tensor([1.0, -1.0, 0.001]).view(3, 1, 1)
+    q, k, v, g = (t.half().cuda() for t in (q, k, v, g))
+    r = oa.attention(q, k, v, [3], [2], grad=g)
+    assert max(r[n].abs().max() for n in ("dq", "dk", "dv")) < 65504
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    o = at.packed_attention(*leaves, at.PackedPlan([3], 2, 1, d, key_lengths=[2]))
+    for n, t in zip(("dq", "dk", "dv"), torch.autograd.grad(o, leaves, g)):
+        near(t, r[n], r[n + "_err"], n)
+
+
+@pytest.mark.parametrize("lengths,keys,heads,kv,d,block,size", [([300, 40], None, 4, 2, 64, 1, 2000.0), ([150], None, 4, 2, 128, 0, 8000.0), ([200], None, 2, 2, 32, 10, 2000.0),
+                                                                ([2, 3], [9000, 5000], 8, 2, 64, 0, 8000.0), ([9000], [9], 3, 1, 64, 0, 50.0)])
+def test_gradients_under_a_loss_scale(lengths, keys, heads, kv, d, block, size):
+    """gradients of thousands in some rows and ordinary ones in others (walks that are split among them)"""
+    q, k, v, g = inputs(lengths, keys, heads, kv, d, F16, 90)
+    q, k = q * 0.5, k * 0.25
+    g[::3] *= size
+    r = oa.attention(q, k, v, lengths, keys, block=block, grad=g)
+    assert max(r[n].abs().max() for n in ("dq", "dk", "dv")) < 65504
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    o = at.packed_attention(*leaves, at.PackedPlan(lengths, heads, kv, d, key_lengths=keys, causal_block=block))
+    for n, t in zip(("dq", "dk", "dv"), torch.autograd.grad(o, leaves, g)):
+        near(t, r[n], r[n + "_err"], n)
