@@ -89,7 +89,8 @@ struct Params {
   View dq, dk, dv;
   char* low;                                     // [q_rows, heads, dim] what the rounding of o left behind, or nothing
   float* lse;                                    // [q_rows, heads]
-  float* delta;                                  // [q_rows, heads]
+  float* delta;                                  // backward, three of [q_rows, heads]: -delta, and what p is made from: exponent m, factor w
+  long row_values;                               // (rows of the plan) * heads: from one of them to the next
   float* part;                                   // split rows: [slot, kv_heads, rows, DP] and behind them [slot, kv_heads, rows, 2]
   const Item* items;
   long n_slots;
@@ -576,10 +577,14 @@ template <typename T, int N> struct Fit {
 };
 
 // dQ: the forward's walk over the keys with dO next to Q.  S^T and dP^T = V dO^T give dS^T in the layout of a B operand; the K tile is
-// read a second time transposed for dQ^T = K^T dS^T.  Writes delta for attn_dkv_kernel on the way.  Split as the forward is; 1.18 PFLOP/s on a
-// training window of 14400 tokens (128 channels).
+// read a second time transposed for dQ^T = K^T dS^T.  Split as the forward is; 1.13 .. 1.18 PFLOP/s (by card) on a training window of 14400 tokens
+// (128 channels).
+// p.  lse has 32 bits: at scores of 10^6 its last bit is 4 % of p, at 10^8 a factor of 250.  So it only says where p is about 1: the walk forms
+// p' = exp2(s c - m), m from lse, and the sum l' of the p' it formed; dQ is divided by l', and attn_dkv_kernel takes p = p' w, w = 1 / l', from the
+// same m and the same bits of s.  m is lowered by what lse can be off (its three roundings and two constants: 4.5 2^-24 of itself), so that l' is 1 at
+// least: at scores of 10^8 it may reach 2^80, which only fp16 minds (Fit).  The sum costs what the products save that start at -delta instead of 0.
 template <typename T, int DP, int NW>
-__global__ __launch_bounds__(NW * 64, 2) void attn_dq_kernel(const Params p) {
+__global__ __launch_bounds__(NW * 64, DP == 128 ? 2 : 3) void attn_dq_kernel(const Params p) {
   using G = Geo<DP>;
   __shared__ __attribute__((aligned(1024))) char smem[4 * G::TILEB];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -612,8 +617,13 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_dq_kernel(const Params p) {
     for (int j = 0; j < 4; ++j) delta += T::lo(gf[s][j]) * (T::lo(of[j]) + T::lo(rf[j])) + T::hi(gf[s][j]) * (T::hi(of[j]) + T::hi(rf[j]));
   }
   delta += other_half(delta);
-  const float lse2 = p.lse[t_ * p.heads + h_] * LOG2E - T::LIFT;
-  if (valid && lane < 32 && it.begin == 0) p.delta[t_ * p.heads + h_] = delta;                         // (the first of a split walk)
+  const float lse2 = p.lse[t_ * p.heads + h_] * LOG2E;
+  const float m = lse2 == -INFINITY ? 0.f : lse2 - fabsf(lse2) * 0x1.2p-22f - T::LIFT;                 // (finite where nothing is seen)
+  if (valid && lane < 32 && it.begin == 0) {                                 // (the first of a split walk)
+    p.delta[t_ * p.heads + h_] = -delta;
+    p.delta[t_ * p.heads + h_ + p.row_values] = m;
+  }
+  float l = 0.f;                                                             // this half's keys only
 
   f32x16 acc[DP / 32];
 #pragma unroll
@@ -652,20 +662,24 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_dq_kernel(const Params p) {
     for (int b = 0; b < 2; ++b) {
       f32x16 s, dp;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.f;
+      for (int i = 0; i < 16; ++i) { s[i] = 0.f; dp[i] = -delta; }
 #pragma unroll
       for (int ks = 0; ks < DP / 16; ++ks) {
         s = T::mfma(frag<DP>(kt, b, ks, lane), qf[ks], s);
         dp = T::mfma(frag<DP>(vt, b, ks, lane), gf[ks], dp);
       }
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] = exp2_fast(fmaf(s[i], p.c, -lse2)) * (dp[i] - delta);
       if (masked) {
         RARE_BRANCH();
         const int end = lim - n0 - 4 * (lane >> 5);
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-          if (b * 32 + 8 * (i / 4) + (i & 3) >= end) s[i] = 0.f;
+          if (b * 32 + 8 * (i / 4) + (i & 3) >= end) { s[i] = -INFINITY; dp[i] = 0.f; }
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[i] = exp2_fast(fmaf(s[i], p.c, -m));
+        l += s[i];
+        s[i] *= dp[i];
       }
       fit(s, acc);
 #pragma unroll
@@ -678,9 +692,12 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_dq_kernel(const Params p) {
       }
     }
   }
-  const float f = p.scale / fit.factor * (1.f / (1 << T::LIFT));
+  l += other_half(l);
   if (it.slot >= 0) {
-    float* out = p.part + (((long)it.slot * p.kv_heads + hk) * (NW * 32) + row) * DP;
+    const long at = ((long)it.slot * p.kv_heads + hk) * (NW * 32) + row;
+    float* out = p.part + at * DP;
+    const float f = 1.f / fit.factor;
+    if (lane < 32) p.part[p.n_slots * p.kv_heads * (NW * 32) * DP + at] = l;
 #pragma unroll
     for (int mb = 0; mb < DP / 32; ++mb)
 #pragma unroll
@@ -689,6 +706,8 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_dq_kernel(const Params p) {
     return;
   }
   if (!valid) return;
+  const float inv = l > 0.f || l != l ? 1.f / l : 0.f, f = p.scale * inv / fit.factor;
+  if (lane < 32) p.delta[t_ * p.heads + h_ + 2 * p.row_values] = inv * (1 << T::LIFT);
   char* op = const_cast<char*>(p.dq.p) + t_ * p.dq.st + h_ * p.dq.sh;
 #pragma unroll
   for (int mb = 0; mb < DP / 32; ++mb)
@@ -711,8 +730,16 @@ __global__ __launch_bounds__(256) void attn_dq_join_kernel(const Params p) {
   const int tok = it.first + row / p.group, head = hk * p.group + row % p.group;
   if (row >= 128 / p.group * p.group || tok >= it.q_len || d >= p.dim || !item_ok(it, p) || (long)it.begin + it.end > p.n_slots) return;
   f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-  for (int i = 0; i < it.end; ++i) sum += *reinterpret_cast<const f32x4*>(p.part + (((long)(it.begin + i) * p.kv_heads + hk) * 128 + row) * DP + d);
-  *reinterpret_cast<u32x2*>(const_cast<char*>(p.dq.p) + (long)(it.q_start + tok) * p.dq.st + (long)head * p.dq.sh + d * 2) = u32x2{T::pack(sum.x, sum.y), T::pack(sum.z, sum.w)};
+  float l = 0.f;
+  for (int i = 0; i < it.end; ++i) {
+    const long slot = ((long)(it.begin + i) * p.kv_heads + hk) * 128 + row;
+    sum += *reinterpret_cast<const f32x4*>(p.part + slot * DP + d);
+    l += p.part[p.n_slots * p.kv_heads * 128 * DP + slot];
+  }
+  const float inv = l > 0.f || l != l ? 1.f / l : 0.f, f = p.scale * inv;
+  if (d == 0) p.delta[(long)(it.q_start + tok) * p.heads + head + 2 * p.row_values] = inv * (1 << T::LIFT);
+  *reinterpret_cast<u32x2*>(const_cast<char*>(p.dq.p) + (long)(it.q_start + tok) * p.dq.st + (long)head * p.dq.sh + d * 2) =
+      u32x2{T::pack(sum.x * f, sum.y * f), T::pack(sum.z * f, sum.w * f)};
 }
 
 // dK, dV: one workgroup holds 64 keys of one key head (128 where head_dim > 64), 32 a wave, and walks over the rows (tokens x group) that see
@@ -726,7 +753,7 @@ template <int DP> struct Dkv {
   static constexpr bool WIDE = DP == 128;                                    // K in LDS as well
   static constexpr int KW = WIDE ? 4 : 2, RW = 2;                            // waves along the keys / along the rows
   static constexpr int WAVES = KW * RW, KEYS = KW * 32, ROWS = RW * 32, TB = ROWS * Geo<DP>::ROWB;
-  static constexpr int LDS = 4 * TB + (WIDE ? 2 : 1) * KEYS * Geo<DP>::ROWB + 5 * ROWS * 4;
+  static constexpr int LDS = 4 * TB + (WIDE ? 2 : 1) * KEYS * Geo<DP>::ROWB + 7 * ROWS * 4;
 };
 
 template <typename T, int DP>
@@ -734,7 +761,7 @@ __global__ __launch_bounds__(Dkv<DP>::WAVES * 64, DP == 128 ? 2 : 3) void attn_d
   using G = Geo<DP>;
   constexpr int TB = Dkv<DP>::TB, DKV_ROWS = Dkv<DP>::ROWS, DKV_KEYS = Dkv<DP>::KEYS, DKV_WAVES = Dkv<DP>::WAVES;
   constexpr bool WIDE = Dkv<DP>::WIDE;
-  extern __shared__ __attribute__((aligned(1024))) char dyn[];               // [buffer][Q, dO], V, [buffer][lse2, delta], tokens of the rows
+  extern __shared__ __attribute__((aligned(1024))) char dyn[];               // [buffer][Q, dO], V (and K), [buffer][m, w, -delta], tokens of the rows
   const int lane = threadIdx.x & 63, wave = (threadIdx.x >> 6) % Dkv<DP>::KW, rw = (threadIdx.x >> 6) / Dkv<DP>::KW;       // 32 keys, 32 rows of a tile
   if (blockIdx.x >= p.blocks) {
     clear_rows<DKV_WAVES * 64>(p.dk, p.clear_k, p.k_rows, p.kv_heads, p.dim, blockIdx.x - p.blocks, gridDim.x - p.blocks);
@@ -748,7 +775,7 @@ __global__ __launch_bounds__(Dkv<DP>::WAVES * 64, DP == 128 ? 2 : 3) void attn_d
   const bool valid = key < it.k_len;
   char* const vtile = dyn + 4 * TB;
   float* const stat = reinterpret_cast<float*>(vtile + (WIDE ? 2 : 1) * DKV_KEYS * G::ROWB);
-  int* const row_tok = reinterpret_cast<int*>(stat + 4 * DKV_ROWS);
+  int* const row_tok = reinterpret_cast<int*>(stat + 6 * DKV_ROWS);
   lds_char* const lds = (lds_char*)dyn;
   const unsigned lds0 = (unsigned)(unsigned long)lds;
   {
@@ -788,23 +815,25 @@ __global__ __launch_bounds__(Dkv<DP>::WAVES * 64, DP == 128 ? 2 : 3) void attn_d
   // the wave.
   auto seen_from = [&](int k) { return p.block ? (int)((unsigned)k / (unsigned)p.block * (unsigned)p.block) - (it.k_len - it.q_len) : 0; };
   const int from = seen_from(key), wave_any = seen_from(it.first + wave * 32), wave_all = seen_from(min(it.first + wave * 32 + 32, it.k_len) - 1);
-  // row statistics: 32 threads hold a row of the next tile each
+  // row statistics: DKV_ROWS threads hold a row of the next tile each
   const int mrow = threadIdx.x, mtok = mrow / p.group, mhead = hk * p.group + mrow % p.group;
-  float m_lse = INFINITY, m_delta = 0.f;
+  float r_m = 0.f, r_w = 0.f, r_delta = 0.f;
   if (mrow < DKV_ROWS) row_tok[mrow] = mtok;
   auto fetch = [&](int t) {
     if (mrow >= DKV_ROWS) return;
     const int tk = it.begin + t * tpt + mtok;
     const bool in = mrow < tpt * p.group && tk < tok_end;
     const long at = (long)(it.q_start + (in ? tk : it.begin)) * p.heads + (in ? mhead : hk * p.group);
-    m_lse = in ? p.lse[at] * LOG2E - T::LIFT : INFINITY;                      // p = 0 in rows that do not exist
-    m_delta = in ? p.delta[at] : 0.f;
+    r_delta = in ? p.delta[at] : 0.f;
+    r_m = in ? p.delta[at + p.row_values] : 0.f;
+    r_w = in ? p.delta[at + 2 * p.row_values] : 0.f;                         // p = 0 in rows that do not exist
   };
   auto park = [&](int t) {
     if (mrow >= DKV_ROWS) return;
-    float* f = stat + (t & 1) * 2 * DKV_ROWS + mrow;
-    f[0] = m_lse;
-    f[DKV_ROWS] = m_delta;
+    float* f = stat + (t & 1) * 3 * DKV_ROWS + mrow;
+    f[0] = r_m;
+    f[DKV_ROWS] = r_w;
+    f[2 * DKV_ROWS] = r_delta;
   };
   auto issue = [&](int t) {
     const unsigned to = lds0 + (t & 1) * 2 * TB;
@@ -828,12 +857,16 @@ __global__ __launch_bounds__(Dkv<DP>::WAVES * 64, DP == 128 ? 2 : 3) void attn_d
     const lds_char* qt = lds + (t & 1) * 2 * TB;
     const lds_char* gt = qt + TB;
     const lds_char* vt = lds + 4 * TB;
-    const float* st = stat + (t & 1) * 2 * DKV_ROWS;
+    const float* st = stat + (t & 1) * 3 * DKV_ROWS;
     const int first_tok = it.begin + t * tpt;
     if (first_tok + tpt > wave_any) {                                        // (else no row of the tile sees a key of the wave)
       f32x16 s, dp;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.f;
+      for (int i4 = 0; i4 < 4; ++i4) {
+        const f32x4 from_delta = *reinterpret_cast<const f32x4*>(st + 2 * DKV_ROWS + rw * 32 + 8 * i4 + 4 * (lane >> 5));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { s[4 * i4 + j] = 0.f; dp[4 * i4 + j] = from_delta[j]; }
+      }
 #pragma unroll
       for (int ks = 0; ks < DP / 16; ++ks) {
         if constexpr (WIDE) s = T::mfma(frag<DP>(qt, rw, ks, lane), frag<DP>(vt + DKV_KEYS * G::ROWB, wave, ks, lane), s);
@@ -844,13 +877,13 @@ __global__ __launch_bounds__(Dkv<DP>::WAVES * 64, DP == 128 ? 2 : 3) void attn_d
 #pragma unroll
       for (int i4 = 0; i4 < 4; ++i4) {
         const int r = rw * 32 + 8 * i4 + 4 * (lane >> 5);
-        const f32x4 lse2 = *reinterpret_cast<const f32x4*>(st + r);
-        const f32x4 delta = *reinterpret_cast<const f32x4*>(st + DKV_ROWS + r);
+        const f32x4 m = *reinterpret_cast<const f32x4*>(st + r);
+        const f32x4 w = *reinterpret_cast<const f32x4*>(st + DKV_ROWS + r);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int i = 4 * i4 + j;
-          s[i] = exp2_fast(fmaf(s[i], p.c, -lse2[j]));
-          dp[i] = s[i] * (dp[i] - delta[j]);
+          s[i] = exp2_fast(fmaf(s[i], p.c, -m[j])) * w[j];
+          dp[i] *= s[i];
         }
         if (masked) {
           RARE_BRANCH();
@@ -1208,12 +1241,12 @@ extern "C" int dh_attn_fwd(const void* q, int64_t q_st, int64_t q_sh, const void
   return dp == 32 ? run_fwd<BF16, 32>(p, *info, items, st) : dp == 64 ? run_fwd<BF16, 64>(p, *info, items, st) : run_fwd<BF16, 128>(p, *info, items, st);
 }
 
-static size_t delta_floats(const dh_attn_info* i) { return ((size_t)i->q_rows * i->heads + 3) / 4 * 4; }
+static size_t row_floats(const dh_attn_info* i) { return ((size_t)i->q_rows * i->heads * 3 + 3) / 4 * 4; }
 extern "C" size_t dh_attn_bwd_workspace_bytes(const dh_attn_info* info) {
   if (!info_ok(info)) return 0;
   // the parts of dQ are joined before those of dK and dV are written
   const size_t dp = pad_dim((int)info->head_dim), keys = dp == 128 ? Dkv<128>::KEYS : Dkv<64>::KEYS;
-  return (delta_floats(info) + std::max((size_t)info->n_dq_slots * 128, (size_t)info->n_dkv_slots * keys * 2) * info->kv_heads * dp) * sizeof(float);
+  return (row_floats(info) + std::max((size_t)info->n_dq_slots * 128 * (dp + 1), (size_t)info->n_dkv_slots * keys * 2 * dp) * info->kv_heads) * sizeof(float);
 }
 
 extern "C" int dh_attn_bwd(const void* grad, int64_t g_st, int64_t g_sh, const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh,
@@ -1240,7 +1273,7 @@ extern "C" int dh_attn_bwd(const void* grad, int64_t g_st, int64_t g_sh, const v
   if (rest_k && (!view_ok(p.dk, k_rows, info->kv_heads, dim) || !view_ok(p.dv, k_rows, info->kv_heads, dim))) return DH_ERR_ARG;
   if (info->n_dkv && (!view_ok(p.k, k_rows, info->kv_heads, dim, true) || !view_ok(p.v, k_rows, info->kv_heads, dim, true) || !view_ok(p.dk, k_rows, info->kv_heads, dim) ||
                       !view_ok(p.dv, k_rows, info->kv_heads, dim))) return DH_ERR_ARG;
-  p.low = (char*)const_cast<void*>(o_low); p.lse = const_cast<float*>(lse); p.delta = (float*)workspace; p.part = (float*)workspace + delta_floats(info);
+  p.low = (char*)const_cast<void*>(o_low); p.lse = const_cast<float*>(lse); p.delta = (float*)workspace; p.row_values = info->q_rows * info->heads; p.part = (float*)workspace + row_floats(info);
   p.kv_heads = (int)info->kv_heads; p.heads = (int)info->heads; p.group = p.heads / p.kv_heads; p.dim = dim; p.block = (int)info->causal_block;
   p.q_rows = (int)q_rows; p.k_rows = (int)k_rows; p.clear_q = clear_rest ? (int)info->q_rows : p.q_rows; p.clear_k = clear_rest ? (int)info->k_rows : p.k_rows; p.scale = scale; p.c = scale * LOG2E;
   const Item* items = reinterpret_cast<const Item*>(plan);

@@ -484,7 +484,7 @@ int dh_reproject_ex(const float* poses, const float* disps, const float* intrins
  *   o = softmax(scale q k^T) v (scale > 0), lse [q_rows, heads] f32 = natural logarithm of the row's sum.
  * Rows behind the last sequence (of o, lse, dq) and behind the last key (of dk, dv) are left as they were, or cleared where clear_rest
  * (o, gradients 0, lse -inf).  Rows of dk, dv between the sequences' keys (k_start with gaps) are left as they were.
- * Scores (scale q.k) up to 10^8 in size.  Values are expected to be finite where a gradient is wanted (rows that see nothing may hold anything).  A non-finite value (q, k or v) reaches the rows that see it and no others.
+ * Scores (scale q.k) up to 10^8 in size, gradients too.  Values are expected to be finite where a gradient is wanted (rows that see nothing may hold anything).  A non-finite value (q, k or v) reaches the rows that see it and no others.
  *
  * dh_attn_plan runs on the HOST: it lays out the work items of one set of lengths.  plan_host NULL: only fills *info (info->ints = ints
  * wanted); else writes plan_host[0 .. info->ints).  The caller copies it to the device and passes it, with *info, to every call on these

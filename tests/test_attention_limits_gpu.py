@@ -47,3 +47,33 @@ def test_gradients_under_a_loss_scale(lengths, keys, heads, kv, d, block, size):
     o = at.packed_attention(*leaves, at.PackedPlan(lengths, heads, kv, d, key_lengths=keys, causal_block=block))
     for n, t in zip(("dq", "dk", "dv"), torch.autograd.grad(o, leaves, g)):
         near(t, r[n], r[n + "_err"], n)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("a,b", [(4, 4), (64, 64), (128, 128), (512, 256), (2048, 1536), (4096, 1536), (4096, 2816)])
+@pytest.mark.parametrize("d,lengths,keys,heads", [(64, [3, 40], [4, 4], 2), (128, [5], [8], 1), (32, [1, 1], [8192, 2048], 8), (128, [2, 1], [16384, 8], 4), (64, [7000], [4], 8)])
+def test_gradients_at_large_scores(d, lengths, keys, heads, a, b, sign, dtype):
+    """all keys are alike, so that each weighs 1 / keys whatever the score is: +- a b sqrt(d), up to 9 10^7.  Lengths are powers of two: the weights
+    are exact in 16 bits, dV is a mean of dO, dQ and dK are what 32-bit sums leave of zero"""
+    m, l = sum(lengths), sum(keys)
+    scale = 64 ** 0.5 / d                                                    # scores of a b 8 for every d
+    q = torch.full((m, heads, d), float(a), dtype=dtype, device="cuda")
+    k = torch.full((l, 1, d), float(sign * b), dtype=dtype, device="cuda")
+    v, g = rand((1, 1, d), dtype, 1).expand(l, 1, d).contiguous(), rand((m, heads, d), dtype, 2)
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    o, lse = at.packed_attention(*leaves, at.PackedPlan(lengths, heads, 1, d, key_lengths=keys), scale=scale, return_lse=True)
+    assert torch.equal(o, v[:1].expand(m, heads, d))                         # a mean of equal numbers
+    dq, dk, dv = (t.double().cpu() for t in torch.autograd.grad(o, leaves, g))
+    u, u32 = oa.half_step(dtype), 2.0 ** -24
+    G, V = g.double().cpu(), v.double().cpu()
+    q0 = k0 = 0
+    for x, y in zip(lengths, keys):
+        # dP and delta are sums of d products each that start alike; delta once more
+        dS = 4 * (d + 8) * u32 * (G[q0:q0 + x].abs() * V[0].abs()).sum(-1).max() / y
+        want, size = G[q0:q0 + x].sum((0, 1)) / y, G[q0:q0 + x].abs().sum((0, 1)) / y
+        err = u * want.abs() + (x * heads + 64) * u32 * size + 2.0 ** -25 + 2.0 ** -28 * size * y
+        assert ((dv[k0:k0 + y, 0] - want).abs() <= err).all(), "dv: %g" % (dv[k0:k0 + y, 0] - want).abs().max()
+        assert dq[q0:q0 + x].abs().max() <= (dS + 2.0 ** -28) * y * scale * b * (1 + u), "dq"
+        assert dk[k0:k0 + y].abs().max() <= (dS + 2.0 ** -28) * x * heads * scale * a * (1 + u), "dk"
+        q0, k0 = q0 + x, k0 + y
