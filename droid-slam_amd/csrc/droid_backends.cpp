@@ -11,7 +11,6 @@
 #include <c10/hip/HIPStream.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
-#include <ATen/MemoryOverlap.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <vector>
 #include <algorithm>
@@ -823,6 +822,67 @@ torch::Tensor attn_input(const torch::Tensor& t, bool keys = false) {
   return ok ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 
+// What a view [rows, heads, channels] with adjacent channels covers: rows x heads pieces of `width` bytes.  at::get_overlap_status decides nothing for
+// views that are not dense, and heads sliced from one projection are not.
+struct Pieces { int64_t p, rows, st, heads, sh, width; };
+Pieces pieces_of(const torch::Tensor& t) {
+  const int64_t size = t.element_size();
+  if (t.numel() == 0) return {0, 0, 0, 0, 0, 0};
+  if (t.dim() != 3) return {(int64_t)t.data_ptr(), 1, 0, 1, 0, t.numel() * size};                      // positions, frequencies, weights: contiguous
+  return {(int64_t)t.data_ptr(), t.size(0), t.size(0) > 1 ? t.stride(0) * size : 0, t.size(1), t.size(1) > 1 ? t.stride(1) * size : 0, t.size(2) * size};
+}
+// is there an m of [lo, hi] with -before < x + m step < behind
+bool hits(int64_t x, int64_t step, int64_t lo, int64_t hi, int64_t before, int64_t behind) {
+  if (step == 0) return lo <= hi && x > -before && x < behind;
+  const int64_t y = -before - x, m = std::max(lo, (y >= 0 ? y / step : -((-y + step - 1) / step)) + 1);
+  return m <= hi && x + m * step < behind;
+}
+constexpr int64_t MOST_PAIRS = 1 << 20;
+// Do two of them share a byte?  Exact where the row strides agree (one row agrees with any) or there are up to 2^20 pairs of rows and heads to look
+// at; otherwise yes as soon as the memory between their ends does.
+bool overlap(Pieces a, Pieces b) {
+  if (!a.rows || !b.rows || !a.heads || !b.heads) return false;
+  const auto end = [](const Pieces& x) { return x.p + (x.rows - 1) * x.st + (x.heads - 1) * x.sh + x.width; };
+  if (end(a) <= b.p || end(b) <= a.p) return false;
+  if (a.rows == 1) a.st = b.st;
+  if (b.rows == 1) b.st = a.st;
+  if (a.heads == 1) a.sh = b.sh;
+  if (b.heads == 1) b.sh = a.sh;
+  const bool rows_alike = a.st == b.st, heads_alike = a.sh == b.sh;
+  if (a.rows > b.rows && !rows_alike) std::swap(a, b);                       // the fewer rows one by one
+  const int64_t n = (rows_alike ? 1 : a.rows) * (heads_alike ? a.heads + b.heads - 1 : std::min(a.heads * b.heads, MOST_PAIRS + 1));
+  if (n > MOST_PAIRS) return true;
+  for (int64_t r = 0; r < (rows_alike ? 1 : a.rows); ++r) {
+    const int64_t x = b.p - (a.p + r * a.st), lo = rows_alike ? -(a.rows - 1) : 0;
+    if (heads_alike) {
+      for (int64_t h = -(a.heads - 1); h < b.heads; ++h)
+        if (hits(x + h * a.sh, b.st, lo, b.rows - 1, b.width, a.width)) return true;
+    } else {
+      for (int64_t g = 0; g < a.heads; ++g)
+        for (int64_t h = 0; h < b.heads; ++h)
+          if (hits(x + h * b.sh - g * a.sh, b.st, lo, b.rows - 1, b.width, a.width)) return true;
+    }
+  }
+  return false;
+}
+// do two elements of one view share their place?
+bool overlaps_itself(const Pieces& a) {
+  if (a.rows > 1 && a.st < a.width) return a.heads > 0;
+  for (int64_t h = 1; h < a.heads; ++h)
+    if (hits(h * a.sh, a.st, -(a.rows - 1), a.rows - 1, a.width, a.width)) return true;
+  return false;
+}
+bool same_pieces(const Pieces& a, const Pieces& b) {
+  return a.p == b.p && a.rows == b.rows && a.st == b.st && a.heads == b.heads && a.sh == b.sh && a.width == b.width;
+}
+// (an input whose channels are not adjacent is copied before anything is written)
+void check_out(const torch::Tensor& out, const char* name) { TORCH_CHECK(!overlaps_itself(pieces_of(out)), name, ": several of its elements lie at the same place"); }
+void check_apart(const torch::Tensor& out, const char* name, const torch::Tensor& in, const char* in_name, bool may_be_same = false) {
+  if (out.numel() == 0 || in.numel() == 0 || (in.dim() == 3 && in.stride(2) != 1)) return;
+  const Pieces a = pieces_of(out), b = pieces_of(in);
+  TORCH_CHECK((may_be_same && same_pieces(a, b)) || !overlap(a, b), name, " overlaps ", in_name, may_be_same ? " without being it" : "");
+}
+
 dh_attn_info attn_info(const torch::Tensor& info) {
   TORCH_CHECK(info.device().is_cpu() && info.scalar_type() == torch::kInt64 && info.is_contiguous() && info.numel() * 8 == (int64_t)sizeof(dh_attn_info),
               "info must be what attention_plan returned");
@@ -873,8 +933,8 @@ std::vector<torch::Tensor> attention_forward(torch::Tensor q, torch::Tensor k, t
   if (out) {
     check_heads(o, "out", q);
     TORCH_CHECK(o.sizes() == q.sizes() && attn_view(o), "out must have q's shape, adjacent channels and 16-byte aligned heads");
-    at::assert_no_internal_overlap(o);
-    at::assert_no_overlap(o, q); at::assert_no_overlap(o, k); at::assert_no_overlap(o, v);
+    check_out(o, "out");
+    check_apart(o, "out", q, "q"); check_apart(o, "out", k, "k"); check_apart(o, "out", v, "v");
   }
   q = attn_input(q); k = attn_input(k, true); v = attn_input(v, true);
   const size_t wsb = dh_attn_fwd_workspace_bytes(&i);
@@ -1001,9 +1061,13 @@ std::vector<torch::Tensor> qk_norm_rope_forward(torch::Tensor q, torch::Tensor k
   check_heads(qo, "q_out", q); check_heads(ko, "k_out", q);
   TORCH_CHECK(qo.sizes() == q.sizes() && ko.sizes() == k.sizes() && (qo.numel() == 0 || qo.stride(2) == 1) && (ko.numel() == 0 || ko.stride(2) == 1),
               "q_out / k_out must have the shapes of q / k and adjacent channels");
-  at::assert_no_internal_overlap(qo); at::assert_no_internal_overlap(ko);
-  at::assert_no_partial_overlap(qo, q); at::assert_no_partial_overlap(ko, k);
-  at::assert_no_overlap(qo, k); at::assert_no_overlap(ko, q); at::assert_no_overlap(qo, ko);
+  if (q_out || k_out) {
+    check_out(qo, "q_out"); check_out(ko, "k_out");
+    check_apart(qo, "q_out", q, "q", true); check_apart(ko, "k_out", k, "k", true);
+    check_apart(qo, "q_out", k, "k"); check_apart(ko, "k_out", q, "q"); check_apart(qo, "q_out", ko, "k_out");
+    for (const torch::Tensor* t : {&positions, &inv_freq, q_weight ? &*q_weight : nullptr, k_weight ? &*k_weight : nullptr})
+      if (t) { check_apart(qo, "q_out", *t, "another input"); check_apart(ko, "k_out", *t, "another input"); }
+  }
   q = rope_input(q); k = rope_input(k);
   rope_status(dh_qk_norm_rope_fwd(TOKEN_VIEW(q), TOKEN_VIEW(k), TOKEN_VIEW(qo), TOKEN_VIEW(ko), positions.data_ptr(), a.pos_type,
                                   inv_freq.data_ptr<float>(), a.sections.data(), (int)a.sections.size(), a.qw, a.kw, a.w_dtype, dt, q.size(0), (int)q.size(1), (int)k.size(1),
@@ -1132,6 +1196,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("reproject", &reproject, "fused reprojection (Python thresholds)");
   m.def("se3_op", &se3_op, "SE3 inv/mul/exp/retr");
   m.def("se3_map", &se3_map, "SE3 act4/adjT");
+  m.def("_token_views_overlap", [](const torch::Tensor& a, const torch::Tensor& b) { return overlap(pieces_of(a), pieces_of(b)); }, "what out= is checked with");
+  m.def("_token_view_overlaps_itself", [](const torch::Tensor& a) { return overlaps_itself(pieces_of(a)); }, "what out= is checked with");
   m.def("attention_plan", &attention_plan, "work items of packed attention for one set of lengths", py::arg("q_lengths"), py::arg("k_lengths"), py::arg("k_starts"),
         py::arg("heads"), py::arg("kv_heads"), py::arg("head_dim"), py::arg("causal_block") = 0);
   m.def("attention_forward", &attention_forward, "packed softmax attention: {o, lse, o_low}", py::arg("q"), py::arg("k"), py::arg("v"), py::arg("plan"), py::arg("info"),

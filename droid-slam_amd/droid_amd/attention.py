@@ -48,7 +48,7 @@ def packed_attention(q, k, v, plan, scale=None, out=None, return_lse=False):
 
     Returns o like q, and with `return_lse` also the logarithm of each row's sum [rows, heads] (float32, not differentiable; what two results
     over different keys are joined with).  A token that sees no key: o = 0, lse = -inf, no gradient.  Rows behind the last sequence: 0 / -inf, and
-    left as they were in an `out` of the caller's (no gradient through `out`)."""
+    left as they were in an `out` of the caller's (no gradient through `out`, which shares no memory with q, k and v)."""
     scale = 1.0 / math.sqrt(plan.head_dim) if scale is None else float(scale)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         if out is not None:
@@ -68,7 +68,8 @@ def qk_norm_rope(q, k, positions, inv_freq, sections, q_weight=None, k_weight=No
     inv_freq    [P] float32: radians a position
     interleaved pairs are (2 i, 2 i + 1) instead of (i, P + i)
     normalize   False: rotation alone
-    out         (q_out, k_out) to write to, possibly q and k themselves or rows of a cache (no gradient)"""
+    out         (q_out, k_out) to write to, possibly q and k themselves or rows of a cache (no gradient; they share no other memory with the
+                inputs or each other)"""
     sections = [int(n) for n in sections]
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
         if out is not None:

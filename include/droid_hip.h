@@ -486,6 +486,8 @@ int dh_reproject_ex(const float* poses, const float* disps, const float* intrins
  * (o, gradients 0, lse -inf).  Rows of dk, dv between the sequences' keys (k_start with gaps) are left as they were.
  * Scores (scale q.k) up to 10^8 in size, gradients too.  Values are expected to be finite where a gradient is wanted (rows that see nothing may hold anything).  A non-finite value (q, k or v) reaches the rows that see it and no others.
  *
+ * Outputs overlap neither inputs nor each other.
+ *
  * dh_attn_plan runs on the HOST: it lays out the work items of one set of lengths.  plan_host NULL: only fills *info (info->ints = ints
  * wanted); else writes plan_host[0 .. info->ints).  The caller copies it to the device and passes it, with *info, to every call on these
  * lengths.  Rows split over their keys (few rows, long key ranges) meet in the workspace.
@@ -521,7 +523,7 @@ int dh_attn_bwd(const void* grad, int64_t g_st, int64_t g_sh, const void* q, int
 /* ------------------------------------------------------------------------------------------------
  * Norm of every query and key head and rotation by the token's position, in one pass, forward and backward.
  *   q, q_out, dq_out, dq [tokens, heads, head_dim], k ... [tokens, kv_heads, head_dim], DH_F16, DH_BF16 or DH_F32; *_st / *_sh = elements
- *   between tokens / heads, >= 0 (channels adjacent).  q_out may be q itself, k_out k itself (the same elements, not shifted ones).
+ *   between tokens / heads, >= 0 (channels adjacent).  q_out may be q itself, k_out k itself (the same elements, not shifted ones); they overlap nothing else.
  *   positions [tokens, n_axes]: pos_type 0 = int32, 1 = int64, 2 = float; inv_freq [sum of sections] f32; 1 <= n_axes <= 4.
  * z = x / sqrt(mean(x^2) + eps) * weight (normalize; weight [head_dim] of w_dtype, NULL = ones) or z = x (no weights then).  The first
  * sections[0] pairs turn by positions[:,0] * inv_freq[pair], the next sections[1] by positions[:,1], ...: (a, b) -> (a cos - b sin,

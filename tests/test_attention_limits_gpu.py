@@ -77,3 +77,28 @@ def test_gradients_at_large_scores(d, lengths, keys, heads, a, b, sign, dtype):
         assert dq[q0:q0 + x].abs().max() <= (dS + 2.0 ** -28) * y * scale * b * (1 + u), "dq"
         assert dk[k0:k0 + y].abs().max() <= (dS + 2.0 ** -28) * x * heads * scale * a * (1 + u), "dk"
         q0, k0 = q0 + x, k0 + y
+
+
+def test_out_over_slices_of_one_buffer():
+    """an out= that shares memory with an input is refused, however the views lie; beside them it may lie in the same buffer"""
+    n, d = 300, 64
+    qkv = rand((n, 24, d), F16, 1)
+    q, k, v = qkv[:, :8], qkv[:, 8:10], qkv[:, 10:12]
+    plan = at.PackedPlan([n], 8, 2, d, causal_block=1)
+    want = at.packed_attention(q, k, v, plan)
+    keep = qkv.clone()
+    for out in (q, qkv[:, 2:10], qkv[:, 10:18], qkv[:, 4:20:2], qkv.view(-1)[8 * d:][:n * 8 * d].view(n, 8, d), qkv.as_strided((n, 8, d), (24 * d, 32, 1), 14 * d),
+                qkv.as_strided((n, 8, d), (0, d, 1), 0), qkv.as_strided((n, 8, d), (8, 24 * d, 1), 14 * d)):
+        with pytest.raises(RuntimeError, match="overlaps|same place"):
+            at.packed_attention(q, k, v, plan, out=out)
+    pos, fr = torch.arange(n, device="cuda"), torch.rand(32, device="cuda")
+    for out in ((qkv[:, 1:9], qkv[:, 12:14]), (qkv[:, 12:20], qkv[:, 9:11]), (qkv[:, 12:20], qkv[:, 19:21]), (qkv[:, 8:16], qkv[:, 16:18]), (qkv[:, 12:20], qkv[:, 6:8]), (q, qkv[:, 7:9])):
+        with pytest.raises(RuntimeError, match="overlaps"):
+            at.qk_norm_rope(q, k, pos, fr, [32], out=out)
+    assert torch.equal(qkv, keep)                                            # nothing was written
+    for out in (qkv[:, 12:20], qkv[:, 13:21]):
+        assert torch.equal(at.packed_attention(q, k, v, plan, out=out), want)
+    turned = [t.clone() for t in at.qk_norm_rope(q, k, pos, fr, [32])]
+    for out in ((qkv[:, 12:20], qkv[:, 20:22]), (q, k)):
+        got = at.qk_norm_rope(q, k, pos, fr, [32], out=out)
+        assert torch.equal(got[0], turned[0]) and torch.equal(got[1], turned[1])
