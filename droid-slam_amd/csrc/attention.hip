@@ -49,6 +49,9 @@ struct F16 {
   using V8 = f16x8;
   // p ~ 1 / (keys) and dS are lifted by 2^4 before they are rounded: 1 / 262144 is still a normal number.  A dS has no bound: see Fit.
   static constexpr int LIFT = 4;
+  // forward: p is 2^TOP where the running maximum was set, 2^(TOP + 8) at most before it is set again (2^15 fits).  Weights down to 2^-21 of the largest
+  // keep fp16's precision, those below 2^-32 count as zero; with TOP = 0 that was 2^-14 and 2^-25, and a tail of thousands of them was lost together
+  static constexpr float TOP = 7.f;
   static constexpr unsigned ONE = 0x3c00, INF = 0x7c00;
   static __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(V8, a), __builtin_bit_cast(V8, b), c, 0, 0, 0);
@@ -63,6 +66,7 @@ struct F16 {
 struct BF16 {
   using V8 = bf16x8;
   static constexpr int LIFT = 0;                 // bf16 has the exponent range of fp32
+  static constexpr float TOP = 0.f;
   static constexpr unsigned ONE = 0x3f80, INF = 0x7f80;
   static __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(V8, a), __builtin_bit_cast(V8, b), c, 0, 0, 0);
@@ -266,8 +270,8 @@ constexpr int CLEAR_BYTES = 1 << 15;             // a workgroup's share
 
 // ------------------------------------------------------------------------------------------------------------- forward
 // One workgroup: NW x 32 rows (NW * 32 / group tokens) of one key head over the keys [begin, end) of its sequence.  Running maximum and sum
-// per row; the accumulator is only rescaled when a maximum grew by more than 2^8 (p <= 256 until then: exact in 32 bits, and a 16-bit p
-// keeps its relative precision).  slot >= 0: the row range is split over the keys, unnormalised sums go to the workspace for attn_join.
+// per row; the accumulator is only rescaled when a maximum grew by more than 2^8 (p <= 2^(TOP + 8) until then: exact in 32 bits, and a 16-bit p
+// keeps its relative precision, in fp16 down to 2^-21 of the largest).  slot >= 0: the row range is split over the keys, unnormalised sums go to the workspace for attn_join.
 // Bound by the matrix cores at the power limit (128 channels: 1.11 PFLOP/s on 19200 tokens, the library's large product 1.25), by the vector
 // units at 64 channels (0.72 on packed clips).
 // How the keys come in: 64 keys a tile, one tile ahead; a lone wave (few rows, bound by memory: 82 us for 32 queries over 358 MB of keys, 4.4 TB/s)
@@ -343,7 +347,8 @@ __global__ __launch_bounds__(NW * 64, NW == 1 ? 1 : DP == 128 ? 2 : 3) void attn
     for (int ks = 0; ks < DP / 16; ++ks) s = T::mfma(frag<DP>(kt, b, ks, lane), qf[ks], s);
     return s;
   };
-  // hides what a row does not see and keeps p at or below 2^8.  Each half of the wave looks at its own keys of a row; only where one of
+  // hides what a row does not see and keeps p at or below 2^(TOP + 8), looking at the exponent that p gets (at scores of 10^8 the maximum's own
+  // rounding is +- 8: the new one is formed in one step).  Each half of the wave looks at its own keys of a row; only where one of
   // them found a maximum that is too large the halves agree on a new one.
   auto settle = [&](f32x16& s, int n0) {
     if (n0 + 32 > wmin) {
@@ -356,10 +361,10 @@ __global__ __launch_bounds__(NW * 64, NW == 1 ? 1 : DP == 128 ? 2 : 3) void attn
     float mx = s[0];
 #pragma unroll
     for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
-    if (__any(mx * p.c > m + 8.f)) {
+    if (__any(fmaf(mx, p.c, -m) > T::TOP + 8.f)) {
       RARE_BRANCH();
-      mx = fmaxf(mx, other_half(mx)) * p.c;
-      const float mn = mx > m + 8.f ? mx : m, a = exp2_fast(m - mn);         // (a row's bits do not depend on its neighbours)
+      mx = fmaxf(mx, other_half(mx));
+      const float mn = fmaf(mx, p.c, -m) > T::TOP + 8.f ? fmaf(mx, p.c, -T::TOP) : m, a = exp2_fast(m - mn);         // (a row's bits do not depend on its neighbours)
       m = mn;
       l *= a;
 #pragma unroll

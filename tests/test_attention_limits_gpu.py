@@ -102,3 +102,21 @@ def test_out_over_slices_of_one_buffer():
     for out in ((qkv[:, 12:20], qkv[:, 20:22]), (q, k)):
         got = at.qk_norm_rope(q, k, pos, fr, [32], out=out)
         assert torch.equal(got[0], turned[0]) and torch.equal(got[1], turned[1])
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("low", [-16.0, -17.40625, -18.5])
+def test_a_long_tail_of_small_weights(low, d, dtype):
+    """one key far above thousands of others: their weights are small one by one and count together (walks that are not split)"""
+    heads, n, rows = 8, 8192, 8960
+    q, k, v = torch.zeros(rows, heads, d, dtype=dtype), torch.zeros(n, heads, d, dtype=dtype), torch.ones(n, heads, d, dtype=dtype)
+    q[..., 0], k[1:, :, 0], v[0] = 1.0, low, 0.0
+    q, k, v = q.cuda(), k.cuda(), v.cuda()
+    plan = at.PackedPlan([rows], heads, heads, d, key_lengths=[n])
+    assert int(plan.info[7]) == 0                                            # (no joins)
+    o, lse = at.packed_attention(q, k, v, plan, scale=1.0, return_lse=True)
+    r = oa.attention(q[:1, :1], k[:, :1], v[:, :1], [1], [n], scale=1.0)
+    assert bool((o == o[:1, :1]).all()) and bool((lse == lse[:1, :1]).all())
+    near(o[:1, :1], r["o"], r["o_err"], "o")
+    near(lse[:1, :1], r["lse"], r["lse_err"], "lse")
