@@ -9,18 +9,16 @@
 // are a few exchanges between neighbours.  The angles belong to the token: a lane computes its sines and cosines once and keeps them for
 // all heads of its token.
 //
-// Angles.  pos * inv_freq is formed in revolutions in 64 bits and reduced to half a turn before it is rounded to 32: at position 10^6 a
-// 32-bit product is off by 0.06 rad, this one by 10^-9.  The hardware's sine and cosine take turns and are as good as 32 bits there.
+// Angles.  pos * inv_freq is formed in revolutions in 64 bits (three roundings: off by 2^-51 of itself at most) and reduced to half a turn there: at
+// position 10^6 a 32-bit product is off by 0.06 rad, this one by 4 10^-10.  16-bit heads: the rest is rounded to 32 bits and goes to the hardware's sine and
+// cosine, which take turns: off by 2.2 10^-7 with the rounding, a 2000th of fp16's half step.  32-bit heads, where that would be three half steps: Taylor's
+// series in 64 bits on an eighth of a turn, rounded once (once for all heads of a token: 10.5 -> 11.1 us at 9000 tokens x 12 heads of 40).
 #include "common.h"
 #include <algorithm>
 #include <string.h>
 
 namespace {
 using namespace dh;
-
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 struct IoF32 {
   static constexpr int SIZE = 4, VMAX = 4;
@@ -87,8 +85,20 @@ template <int V, bool PAIRS_ADJACENT> struct Lane {
   __device__ __forceinline__ int pair(int i) const { return PAIRS_ADJACENT ? lo / 2 + i : lo + i; }
 };
 
+// sin and cos of `rev` turns, |rev| <= 1/2, rounded to 32 bits once: the nearest quarter turn is taken off, and the series to x^13 and x^12 are off by
+// 4 10^-13 where |x| <= pi / 4
+__device__ __forceinline__ void sincos_turns(double rev, float& s, float& c) {
+  const int n = (int)rint(4. * rev);
+  const double x = (rev - .25 * n) * 6.28318530717958647693, y = x * x;
+  const double si = x + x * y * (-1. / 6 + y * (1. / 120 + y * (-1. / 5040 + y * (1. / 362880 + y * (-1. / 39916800 + y * (1. / 6227020800.))))));
+  const double co = 1. + y * (-1. / 2 + y * (1. / 24 + y * (-1. / 720 + y * (1. / 40320 + y * (-1. / 3628800 + y * (1. / 479001600.))))));
+  const float a = (float)(n & 1 ? co : si), b = (float)(n & 1 ? si : co);
+  s = n & 2 ? -a : a;
+  c = (n + 1) & 2 ? -b : b;
+}
+
 template <int V> struct Turn { float c[V], s[V]; };
-template <int V, bool ADJ> __device__ __forceinline__ Turn<V> turn_of(const RopeParams& p, const Lane<V, ADJ>& ln, long tok) {
+template <typename Io, int V, bool ADJ> __device__ __forceinline__ Turn<V> turn_of(const RopeParams& p, const Lane<V, ADJ>& ln, long tok) {
   Turn<V> t;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
@@ -103,6 +113,10 @@ template <int V, bool ADJ> __device__ __forceinline__ Turn<V> turn_of(const Rope
       const double x = p.pos_type == 0 ? (double)reinterpret_cast<const int*>(p.pos)[at]
                      : p.pos_type == 1 ? (double)reinterpret_cast<const long*>(p.pos)[at] : (double)reinterpret_cast<const float*>(p.pos)[at];
       const double rev = x * ((double)p.inv_freq[j] * 0.15915494309189533577);
+      if constexpr (Io::SIZE == 4) {
+        sincos_turns(rev - rint(rev), t.s[i], t.c[i]);
+        continue;
+      }
       const float turn = (float)(rev - rint(rev));                           // half a turn at most
       t.s[i] = __builtin_amdgcn_sinf(turn);                                  // v_sin_f32, v_cos_f32: argument in turns, off by 1.25e-7 at most
       t.c[i] = __builtin_amdgcn_cosf(turn);                                  // on [-1/2, 1/2] (all 2^22 multiples of 2^-22 compared with 64 bits)
@@ -150,7 +164,7 @@ __global__ __launch_bounds__(256, 4) void rope_fwd_kernel(const RopeParams p) {
   const Lane<V, ADJ> ln(p, lane & ((1 << p.shift) - 1));
   const bool on = ln.on && tok < p.tokens;
   const long tk = tok < p.tokens ? tok : p.tokens - 1;
-  const Turn<V> t = turn_of<V, ADJ>(p, ln, tk);
+  const Turn<V> t = turn_of<Io, V, ADJ>(p, ln, tk);
   const int h_from = blockIdx.y * p.chunk, h_to = h_from + p.chunk;
 #pragma unroll
   for (int n = 0; n < 2; ++n) {
@@ -216,7 +230,7 @@ __global__ __launch_bounds__(256) void rope_bwd_kernel(const RopeParams p) {
     const long tok = t0 + wave * slots + (lane >> p.shift);
     const bool on = ln.on && tok < p.tokens;
     const long tk = tok < p.tokens ? tok : p.tokens - 1;
-    const Turn<V> t = turn_of<V, ADJ>(p, ln, tk);
+    const Turn<V> t = turn_of<Io, V, ADJ>(p, ln, tk);
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
       const int base = n ? p.heads[0] : 0;

@@ -528,7 +528,8 @@ int dh_attn_bwd(const void* grad, int64_t g_st, int64_t g_sh, const void* q, int
  * z = x / sqrt(mean(x^2) + eps) * weight (normalize; weight [head_dim] of w_dtype, NULL = ones) or z = x (no weights then).  The first
  * sections[0] pairs turn by positions[:,0] * inv_freq[pair], the next sections[1] by positions[:,1], ...: (a, b) -> (a cos - b sin,
  * a sin + b cos); with P = sum of sections a pair is (i, P + i), or (2i, 2i + 1) where `interleaved`; channels from 2 P on do not turn.
- * Angles are exact to 32 bits at any position.  head_dim even, up to 256 (above 128 the halves must be even: DH_ERR_UNSUPPORTED).
+ * An angle is off by 2^-51 of itself (64-bit product, reduced there), its sine and cosine by half a step of 32 bits (DH_F32) or 2.2e-7 (16-bit types).
+ * head_dim even, up to 256 (above 128 the halves must be even: DH_ERR_UNSUPPORTED).
  * Backward: x is only read where `normalize`; dq_weight / dk_weight [head_dim] of w_dtype or NULL; no atomics. */
 int dh_qk_norm_rope_fwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh,
                         void* q_out, int64_t qo_st, int64_t qo_sh, void* k_out, int64_t ko_st, int64_t ko_sh,

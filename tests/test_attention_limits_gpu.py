@@ -120,3 +120,22 @@ def test_a_long_tail_of_small_weights(low, d, dtype):
     assert bool((o == o[:1, :1]).all()) and bool((lse == lse[:1, :1]).all())
     near(o[:1, :1], r["o"], r["o_err"], "o")
     near(lse[:1, :1], r["lse"], r["lse_err"], "lse")
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_angles_of_32_bit_features(interleaved):
+    """(1, 0) turns into (cos, sin): nothing is rounded but the sine and the cosine themselves, by half a step"""
+    n, d = 20000, 64
+    x = torch.zeros(n, 1, d, device="cuda")
+    x[..., 0:d:2 if interleaved else 1][..., :d // 2] = 1.0
+    if not interleaved:
+        x[..., d // 2:] = 0.0
+    pos = torch.randint(-3000000, 3000000, (n,), generator=torch.Generator().manual_seed(1)).cuda()
+    pos[:3000] = torch.arange(3000, device="cuda")
+    fr = (10000.0 ** (-torch.arange(d // 2) / (d // 2))).float().cuda()
+    y, _ = at.qk_norm_rope(x, x[:, :0], pos, fr, [d // 2], normalize=False, interleaved=interleaved)
+    ang = pos.double()[:, None] * fr.double()
+    c, s = (y[:, 0, 0::2], y[:, 0, 1::2]) if interleaved else (y[:, 0, :d // 2], y[:, 0, d // 2:])
+    for got, want in ((c, ang.cos()), (s, ang.sin())):
+        # a position times a frequency keeps 53 bits: 3 10^6 2^-52 beside the half step
+        assert bool(((got.double() - want).abs() <= 2.0 ** -24 * want.abs() + 3e6 * 2.0 ** -51).all())
