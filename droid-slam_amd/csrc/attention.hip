@@ -220,6 +220,10 @@ __host__ __device__ __forceinline__ int keys_seen(int i, int q_len, int k_len, i
   return e < (unsigned)k_len ? (int)e : k_len;
 }
 
+// what a row's sum is multiplied by: 1 / l, and zero where nothing is seen.  Where something is, l = 0 says that every score is -inf (a maximum's own p
+// is one): there is no softmax of that
+__device__ __forceinline__ float row_factor(float l, int seen) { return seen <= 0 ? 0.f : l == 0.f ? NAN : 1.f / l; }
+
 __device__ __forceinline__ bool item_ok(const Item& it, const Params& p) {   // (holds for a plan of dh_attn_plan with these tensors)
   return it.q_start >= 0 && it.q_len >= 0 && it.k_start >= 0 && it.k_len >= 0 && it.first >= 0 && it.begin >= 0 &&
          (long)it.q_start + it.q_len <= p.q_rows && (long)it.k_start + it.k_len <= p.k_rows;
@@ -481,7 +485,7 @@ __global__ __launch_bounds__(NW * 64, NW == 1 ? 1 : DP == 128 ? 2 : 3) void attn
     return;
   }
   if (!valid) return;
-  const float inv = l > 0.f || l != l ? 1.f / l : 0.f;                       // nothing seen: zero (NaN stays NaN)
+  const float inv = row_factor(l, lim);
   char* op = const_cast<char*>(p.o.p) + (long)(it.q_start + tok) * p.o.st + (long)head * p.o.sh;
   char* lp = p.low + ((long)(it.q_start + tok) * p.heads + head) * p.dim * 2;
 #pragma unroll
@@ -539,7 +543,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const Params p, int rows
   }
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) l += __shfl_xor(l, off, 64);
-  const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+  const float inv = row_factor(l, keys_seen(tok, it.q_len, it.k_len, p.block));
   unsigned short* op = reinterpret_cast<unsigned short*>(const_cast<char*>(p.o.p) + (long)(it.q_start + tok) * p.o.st + (long)head * p.o.sh);
 #pragma unroll
   for (int k = 0; k < DP / 32; ++k)

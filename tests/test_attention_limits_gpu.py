@@ -139,3 +139,20 @@ def test_angles_of_32_bit_features(interleaved):
     for got, want in ((c, ang.cos()), (s, ang.sin())):
         # a position times a frequency keeps 53 bits: 3 10^6 2^-52 beside the half step
         assert bool(((got.double() - want).abs() <= 2.0 ** -24 * want.abs() + 3e6 * 2.0 ** -51).all())
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("lengths,keys", [([5], [5]), ([1, 3], [9000, 3])])
+def test_rows_whose_scores_are_all_minus_infinity(lengths, keys, dtype):
+    """keys of -inf under positive queries: there is no softmax of that, in a split row neither; others do not change"""
+    q, k, v, _ = inputs(lengths, keys, 2, 1, 64, dtype, 3)
+    q = q.abs()
+    if keys[0] == 5:
+        k[0] = -float("inf")                                                 # token 0 sees only this key
+        o, lse = at.packed_attention(q, k, v, at.PackedPlan(lengths, 2, 1, 64, causal_block=1), return_lse=True)
+        assert bool(o[0].isnan().all()) and bool(torch.isfinite(o[1:]).all())
+    else:
+        k[:9000] = -float("inf")
+        o, lse = at.packed_attention(q, k, v, at.PackedPlan(lengths, 2, 1, 64, key_lengths=keys), return_lse=True)
+        assert bool(o[0].isnan().all()) and bool(torch.isfinite(o[1:]).all())
+    assert bool((lse[0] == -float("inf")).all())
