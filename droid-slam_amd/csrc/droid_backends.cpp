@@ -14,6 +14,7 @@
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <vector>
 #include <algorithm>
+#include <unordered_set>
 #include "../../include/droid_hip.h"
 
 namespace {
@@ -974,15 +975,28 @@ std::vector<torch::Tensor> attention_backward(torch::Tensor grad, torch::Tensor 
 }
 
 // A leaf keeps the stream that its gradient was first wanted on for as long as a graph of it lives; autograd would join that stream into a
-// capture, which ends the process.  Refused instead, before anything is recorded.
+// capture, which ends the process.  Refused instead, before anything is recorded, for every leaf that the inputs come from.
 void refuse_leaves_of_other_streams(std::initializer_list<const torch::Tensor*> inputs, const char* what) {
+  const c10::DeviceGuard guard((*inputs.begin())->device());
   if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+  std::vector<torch::autograd::Node*> todo;
+  std::unordered_set<torch::autograd::Node*> seen;
+  const auto visit = [&](torch::autograd::Node* n) { if (n && seen.insert(n).second) todo.push_back(n); };
+  std::vector<std::shared_ptr<torch::autograd::Node>> held;                  // (what the tensors give may be theirs alone)
   for (const torch::Tensor* t : inputs) {
-    if (!t || !t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
-    const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
-    const auto stream = node ? node->stream() : c10::nullopt;
-    TORCH_CHECK(!stream || *stream == c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t->get_device()).unwrap(), what,
-                ": this stream is being captured, and a graph of the same leaves lives on another one; drop it first");
+    if (!t || !t->defined() || !t->requires_grad()) continue;
+    held.push_back(t->is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(*t) : t->grad_fn());
+    visit(held.back().get());
+  }
+  while (!todo.empty()) {
+    torch::autograd::Node* n = todo.back();
+    todo.pop_back();
+    if (n->next_edges().empty()) {                                           // the end of a path: a leaf's accumulator, or a node without inputs that want a gradient
+      const auto stream = n->stream();
+      TORCH_CHECK(!stream || *stream == c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(stream->device_index()).unwrap(), what,
+                  ": this stream is being captured, and a graph of the same leaves lives on another one; drop it first");
+    }
+    for (const auto& e : n->next_edges()) visit(e.function.get());
   }
 }
 

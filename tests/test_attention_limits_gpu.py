@@ -156,3 +156,33 @@ def test_rows_whose_scores_are_all_minus_infinity(lengths, keys, dtype):
         o, lse = at.packed_attention(q, k, v, at.PackedPlan(lengths, 2, 1, 64, key_lengths=keys), return_lse=True)
         assert bool(o[0].isnan().all()) and bool(torch.isfinite(o[1:]).all())
     assert bool((lse[0] == -float("inf")).all())
+
+
+def test_capture_beside_a_living_graph_of_a_sliced_leaf_is_refused():
+    """heads sliced from one leaf, and what is computed from a leaf before the call: the accumulator lives on the eager stream, autograd would end the process"""
+    n, d = 40, 64
+    qkv, g = rand((n, 8, d), BF16, 1).requires_grad_(), rand((n, 4, d), BF16, 2)
+    w = torch.ones(d, device="cuda", requires_grad=True)
+    plan = at.PackedPlan([n], 4, 2, d, causal_block=1)
+    pos, fr = torch.arange(n, device="cuda", dtype=torch.int32), torch.rand(32, device="cuda")
+
+    def step(x, u):
+        q, k = at.qk_norm_rope(x[:, :4], x[:, 4:6], pos, fr, [32], u, u)
+        return at.packed_attention(q, k, x[:, 6:], plan)
+
+    alive = step(qkv, w * 2)
+    for call in (lambda: at.packed_attention(qkv[:, :4], qkv[:, 4:6], qkv[:, 6:], plan), lambda: at.qk_norm_rope(qkv.detach()[:, :4], qkv.detach()[:, 4:6], pos, fr, [32], w * 2),
+                 lambda: at.qk_norm_rope(qkv[:, :4], qkv[:, 4:6], pos, fr, [32]), lambda: step(qkv * 1, w)):
+        with pytest.raises(RuntimeError, match="captured"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                call()
+    want = torch.autograd.grad(alive, (qkv, w), g)
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(step(qkv, w * 2), (qkv, w), g)
+    for _ in range(3):
+        graph.replay()
+        step(qkv.detach(), w.detach() * 2)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
