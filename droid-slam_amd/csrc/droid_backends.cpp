@@ -804,6 +804,10 @@ int token_dtype(const torch::Tensor& t, const char* name, bool allow_f32) {
   TORCH_CHECK(false, name, allow_f32 ? " must be float16, bfloat16 or float32" : " must be float16 or bfloat16");
   return -1;
 }
+// (a tangent would be dropped in silence)
+void check_no_tangents(std::initializer_list<const torch::Tensor*> tensors) {
+  for (const torch::Tensor* t : tensors) TORCH_CHECK(!t || !t->defined() || !t->_fw_grad(0).defined(), "an input carries a tangent: the token operators have no forward-mode derivative");
+}
 void check_heads(const torch::Tensor& t, const char* name, const torch::Tensor& like) {
   TORCH_CHECK(t.is_cuda(), name, " must be a ROCm device tensor (droid_backends has no CPU path)");
   TORCH_CHECK(t.dim() == 3, name, " must be [rows, heads, head_dim]");
@@ -911,6 +915,7 @@ std::vector<torch::Tensor> attention_plan(const std::vector<int64_t>& q_len, con
 }
 
 void check_attn(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& plan, const dh_attn_info& i, const char* what) {
+  check_no_tangents({&q, &k, &v});
   check_heads(q, "q", q); check_heads(k, "k", q); check_heads(v, "v", q);
   TORCH_CHECK(q.size(1) == i.heads && k.size(1) == i.kv_heads && q.size(2) == i.head_dim && k.size(2) == i.head_dim && v.sizes() == k.sizes(), what,
               ": q must be [rows, ", i.heads, ", ", i.head_dim, "], k and v [rows, ", i.kv_heads, ", ", i.head_dim, "] as the plan says");
@@ -952,6 +957,7 @@ std::vector<torch::Tensor> attention_backward(torch::Tensor grad, torch::Tensor 
                                               c10::optional<torch::Tensor> low, torch::Tensor plan, torch::Tensor info, double scale) {
   const dh_attn_info i = attn_info(info);
   check_attn(q, k, v, plan, i, "attention_backward");
+  check_no_tangents({&grad});
   check_heads(o, "o", q); check_heads(grad, "grad", q);
   TORCH_CHECK(o.sizes() == q.sizes() && grad.sizes() == q.sizes(), "attention_backward: o and grad must have q's shape");
   TORCH_CHECK(lse.device() == q.device() && lse.scalar_type() == torch::kFloat32 && lse.is_contiguous() && lse.dim() == 2 && lse.size(0) == q.size(0) && lse.size(1) == q.size(1),
@@ -977,6 +983,7 @@ std::vector<torch::Tensor> attention_backward(torch::Tensor grad, torch::Tensor 
 // A leaf keeps the stream that its gradient was first wanted on for as long as a graph of it lives; autograd would join that stream into a
 // capture, which ends the process.  Refused instead, before anything is recorded, for every leaf that the inputs come from.
 void refuse_leaves_of_other_streams(std::initializer_list<const torch::Tensor*> inputs, const char* what) {
+  if (!(*inputs.begin())->is_cuda()) return;                                 // (refused further on)
   const c10::DeviceGuard guard((*inputs.begin())->device());
   if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
   std::vector<torch::autograd::Node*> todo;
@@ -1025,6 +1032,7 @@ std::vector<torch::Tensor> packed_attention(torch::Tensor q, torch::Tensor k, to
 struct RopeArgs { std::vector<int> sections; int pos_type, w_dtype; const void *qw, *kw; };
 RopeArgs rope_args(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& positions, const torch::Tensor& inv_freq, const std::vector<int64_t>& sections,
                    const c10::optional<torch::Tensor>& q_weight, const c10::optional<torch::Tensor>& k_weight, bool normalize, double eps) {
+  check_no_tangents({&q, &k, &positions, &inv_freq, q_weight ? &*q_weight : nullptr, k_weight ? &*k_weight : nullptr});
   check_heads(q, "q", q); check_heads(k, "k", q);
   TORCH_CHECK(k.size(0) == q.size(0) && k.size(2) == q.size(2), "q and k must have the same tokens and head_dim");
   const int64_t d = q.size(2);
@@ -1094,6 +1102,7 @@ std::vector<torch::Tensor> qk_norm_rope_backward(torch::Tensor dq_out, torch::Te
                                                  const std::vector<int64_t>& sections, c10::optional<torch::Tensor> q_weight, c10::optional<torch::Tensor> k_weight,
                                                  bool normalize, double eps, bool interleaved) {
   const RopeArgs a = rope_args(q, k, positions, inv_freq, sections, q_weight, k_weight, normalize, eps);
+  check_no_tangents({&dq_out, &dk_out});
   check_heads(dq_out, "dq_out", q); check_heads(dk_out, "dk_out", q);
   TORCH_CHECK(dq_out.sizes() == q.sizes() && dk_out.sizes() == k.sizes(), "the gradients must have the shapes of q and k");
   const int dt = token_dtype(q, "q", true);

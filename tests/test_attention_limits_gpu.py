@@ -186,3 +186,16 @@ def test_capture_beside_a_living_graph_of_a_sliced_leaf_is_refused():
         step(qkv.detach(), w.detach() * 2)
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_forward_mode_is_refused():
+    from torch.autograd import forward_ad as fw
+    x, w, pos, fr = rand((8, 2, 64), F16, 1), torch.ones(64, device="cuda"), torch.arange(8.0, device="cuda"), torch.ones(32, device="cuda")
+    plan = at.PackedPlan([8], 2, 2, 64)
+    with fw.dual_level():
+        dual = lambda t: fw.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for call in (lambda: at.packed_attention(x, x, dual(x), plan), lambda: at.packed_attention(dual(x.clone().requires_grad_()), x, x, plan),
+                     lambda: at.qk_norm_rope(x, x, pos, fr, [32], dual(w)), lambda: at.qk_norm_rope(x, x, dual(pos), fr, [32]), lambda: at.qk_norm_rope(x, x, pos, dual(fr), [32])):
+            with pytest.raises(RuntimeError, match="tangent"):
+                call()
+        assert at.packed_attention(x, x, x, plan).shape == x.shape

@@ -12,6 +12,7 @@ for p in (ROOT, os.path.join(ROOT, "droid-slam_amd")):
         sys.path.insert(0, p)
 
 import droid_backends as db  # noqa: E402
+from droid_amd import attention as at  # noqa: E402
 
 
 def places(t):
@@ -49,3 +50,19 @@ def test_heads_of_one_projection():
     slots = torch.empty(2, 5000, 64, dtype=torch.float16).transpose(0, 1)   # heads outside rows
     assert db._token_views_overlap(slots[:100], slots[50:60]) and not db._token_views_overlap(slots[:100], slots[100:])
     assert db._token_views_overlap(qkv[:, :8], qkv.view(-1)[:12 * 100000 * 64 // 2].view(-1, 4, 64))       # (strides not alike, many rows: taken to overlap)
+
+
+@pytest.mark.parametrize("wants_gradient", [False, True])
+def test_forward_mode_is_refused(wants_gradient):
+    """a tangent is not dropped in silence"""
+    from torch.autograd import forward_ad as fw
+    x, tangent = torch.zeros(4, 2, 32, dtype=torch.float16), torch.ones(4, 2, 32, dtype=torch.float16)
+    plan = at.PackedPlan([4], 2, 2, 32, device="cpu")
+    with fw.dual_level():
+        dual = fw.make_dual(x.clone().requires_grad_() if wants_gradient else x, tangent)
+        for a in ((dual, x, x), (x, dual, x), (x, x, dual)):
+            with pytest.raises(RuntimeError, match="tangent"):
+                at.packed_attention(*a, plan)
+        for a in ((dual, x), (x, dual)):
+            with pytest.raises(RuntimeError, match="tangent"):
+                at.qk_norm_rope(*a, torch.arange(4), torch.ones(16), [16])
