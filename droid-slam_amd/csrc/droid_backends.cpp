@@ -881,7 +881,14 @@ bool same_pieces(const Pieces& a, const Pieces& b) {
   return a.p == b.p && a.rows == b.rows && a.st == b.st && a.heads == b.heads && a.sh == b.sh && a.width == b.width;
 }
 // (an input whose channels are not adjacent is copied before anything is written)
-void check_out(const torch::Tensor& out, const char* name) { TORCH_CHECK(!overlaps_itself(pieces_of(out)), name, ": several of its elements lie at the same place"); }
+void check_out(const torch::Tensor& out, const char* name) {
+  TORCH_CHECK(!overlaps_itself(pieces_of(out)), name, ": several of its elements lie at the same place");
+  TORCH_CHECK(!(at::GradMode::is_enabled() && out.requires_grad()) && !out._fw_grad(0).defined(), name, " wants a gradient or carries a tangent: what is written to it has none");
+}
+// written in place: autograd has to see that a tensor which it kept for a backward pass is another one now
+void mark_written(const torch::Tensor& out) {
+  if (!out.is_inference()) out.unsafeGetTensorImpl()->bump_version();
+}
 void check_apart(const torch::Tensor& out, const char* name, const torch::Tensor& in, const char* in_name, bool may_be_same = false) {
   if (out.numel() == 0 || in.numel() == 0 || (in.dim() == 3 && in.stride(2) != 1)) return;
   const Pieces a = pieces_of(out), b = pieces_of(in);
@@ -948,6 +955,7 @@ std::vector<torch::Tensor> attention_forward(torch::Tensor q, torch::Tensor k, t
   if (wsb) ws = torch::empty({(int64_t)wsb}, q.options().dtype(torch::kUInt8));
   check_status(dh_attn_fwd(TOKEN_VIEW(q), TOKEN_VIEW(k), TOKEN_VIEW(v), TOKEN_VIEW(o), for_backward ? low.data_ptr() : nullptr, lse.data_ptr<float>(),
                            plan.data_ptr<int32_t>(), &i, dt, q.size(0), k.size(0), (float)scale, !out, wsb ? ws.data_ptr() : nullptr, wsb, stream_of(q)), "attention_forward");
+  if (out) mark_written(o);
   if (out && q.size(0) > i.q_rows) lse.narrow(0, i.q_rows, q.size(0) - i.q_rows).fill_(-std::numeric_limits<float>::infinity());
   return {o, lse, low};
 }
@@ -1094,6 +1102,8 @@ std::vector<torch::Tensor> qk_norm_rope_forward(torch::Tensor q, torch::Tensor k
   rope_status(dh_qk_norm_rope_fwd(TOKEN_VIEW(q), TOKEN_VIEW(k), TOKEN_VIEW(qo), TOKEN_VIEW(ko), positions.data_ptr(), a.pos_type,
                                   inv_freq.data_ptr<float>(), a.sections.data(), (int)a.sections.size(), a.qw, a.kw, a.w_dtype, dt, q.size(0), (int)q.size(1), (int)k.size(1),
                                   (int)q.size(2), normalize, (float)eps, interleaved, stream_of(q)), "qk_norm_rope_forward");
+  if (q_out) mark_written(qo);
+  if (k_out) mark_written(ko);
   return {qo, ko};
 }
 

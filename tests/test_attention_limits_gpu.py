@@ -199,3 +199,32 @@ def test_forward_mode_is_refused():
             with pytest.raises(RuntimeError, match="tangent"):
                 call()
         assert at.packed_attention(x, x, x, plan).shape == x.shape
+
+
+def test_out_is_seen_by_autograd():
+    """what is written through out= is a new value: a backward pass that kept the old one says so; an out= that wants a gradient itself is refused"""
+    n, d = 20, 64
+    q, k, v, g = inputs([n], None, 4, 2, d, F16, 7)
+    pos, fr, plan = torch.arange(n, device="cuda"), torch.rand(32, device="cuda"), at.PackedPlan([n], 4, 2, d)
+    a, w = torch.ones_like(q).requires_grad_(), torch.ones_like(k).requires_grad_()
+    kept = [(a * q).sum(), (w * k).sum()]
+    with torch.no_grad():
+        at.qk_norm_rope(q, k, pos, fr, [32], out=(q, k))
+    for t in kept:
+        with pytest.raises(RuntimeError, match="inplace"):
+            t.backward()
+    buf = torch.zeros(n, 8, d, dtype=F16, device="cuda")
+    kept = (torch.ones_like(buf).requires_grad_() * buf).sum()
+    with torch.no_grad():
+        at.packed_attention(q, k, v, plan, out=buf[:, 2:6])                  # (a view: the whole buffer is another one)
+    with pytest.raises(RuntimeError, match="inplace"):
+        kept.backward()
+    leaf = torch.zeros_like(q).requires_grad_()
+    for call in (lambda: at.packed_attention(q, k, v, plan, out=leaf), lambda: at.qk_norm_rope(q, k, pos, fr, [32], out=(leaf, torch.empty_like(k)))):
+        with pytest.raises(RuntimeError, match="gradient"):
+            call()
+        with torch.no_grad():
+            call()
+    with torch.inference_mode():
+        out = torch.empty_like(q)
+        assert torch.equal(at.packed_attention(q, k, v, plan, out=out), at.packed_attention(q, k, v, plan))
