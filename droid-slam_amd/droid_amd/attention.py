@@ -65,12 +65,14 @@ def qk_norm_rope(q, k, positions, inv_freq, sections, q_weight=None, k_weight=No
 
     positions   [tokens, axes] int32, int64 or float32: (keyframe, row, column) or fewer / more axes
     sections    pairs of channels that turn with each axis; their sum P is at most head_dim / 2, channels from 2 P on do not turn
-    inv_freq    [P] float32: radians a position
+    inv_freq    [P] float32: radians a position (positions and inv_freq get no gradient; ones that want one are refused)
     interleaved pairs are (2 i, 2 i + 1) instead of (i, P + i)
     normalize   False: rotation alone
     out         (q_out, k_out) to write to, possibly q and k themselves or rows of a cache (no gradient; they share no other memory with the
                 inputs or each other)"""
     sections = [int(n) for n in sections]
+    if torch.is_grad_enabled() and (positions.requires_grad or inv_freq.requires_grad):
+        raise RuntimeError("qk_norm_rope: positions and inv_freq get no gradient; detach them")
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
         if out is not None:
             raise RuntimeError("qk_norm_rope: out= takes no gradient; leave it out or use torch.no_grad()")

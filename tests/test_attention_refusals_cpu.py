@@ -66,3 +66,14 @@ def test_forward_mode_is_refused(wants_gradient):
         for a in ((dual, x), (x, dual)):
             with pytest.raises(RuntimeError, match="tangent"):
                 at.qk_norm_rope(*a, torch.arange(4), torch.ones(16), [16])
+
+
+def test_gradients_that_nobody_forms_are_refused():
+    """learned frequencies or positions would stay where they are in silence"""
+    x, pos, fr = torch.zeros(4, 2, 32, dtype=torch.float16), torch.arange(4.0), torch.ones(16)
+    for a in ((pos.clone().requires_grad_(), fr), (pos, fr.clone().requires_grad_())):
+        for q in (x, x.clone().requires_grad_()):
+            with pytest.raises(RuntimeError, match="no gradient"):
+                at.qk_norm_rope(q, x, *a, [16])
+        with torch.no_grad(), pytest.raises(RuntimeError, match="device tensor"):
+            at.qk_norm_rope(x, x, *a, [16])
