@@ -1068,12 +1068,15 @@ template <typename T, int DP> int run_bwd(Params p, const dh_attn_info& info, co
   return DH_OK;
 }
 
+constexpr long MAX_THREADS = 0xffffffffl;         // of one launch
+
 bool info_ok(const dh_attn_info* i) {
   if (!i || !heads_ok(i->heads, i->kv_heads, i->head_dim) || i->causal_block < 0 || i->causal_block > MAX_ROWS || (i->waves != 1 && i->waves != 4)) return false;
+  const int64_t threads[3] = {i->waves * 64, 256, (pad_dim((int)i->head_dim) == 128 ? Dkv<128>::WAVES : Dkv<64>::WAVES) * 64};
   const int64_t items[3] = {i->n_fwd, i->n_dq, i->n_dkv}, joins[3] = {i->n_join, i->n_dq_join, i->n_dkv_join}, slots[3] = {i->n_slots, i->n_dq_slots, i->n_dkv_slots};
   int64_t n = 0;
   for (int k = 0; k < 3; ++k) {
-    if (items[k] < 0 || items[k] > INT_MAX / 8 || items[k] * i->kv_heads > INT_MAX - 1024 || joins[k] < 0 || joins[k] * i->kv_heads > 65535 || slots[k] < 0 || slots[k] > items[k]) return false;
+    if (items[k] < 0 || items[k] > INT_MAX / 8 || (items[k] * i->kv_heads + 1024) * threads[k] > MAX_THREADS || joins[k] < 0 || joins[k] * i->kv_heads > 65535 || slots[k] < 0 || slots[k] > items[k]) return false;
     n += items[k] + joins[k];
   }
   return i->ints == 8 * n && i->q_rows >= 0 && i->k_rows >= 0 && i->q_rows <= MAX_ROWS && i->k_rows <= MAX_ROWS;

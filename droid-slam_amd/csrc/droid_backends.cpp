@@ -913,7 +913,7 @@ std::vector<torch::Tensor> attention_plan(const std::vector<int64_t>& q_len, con
   dh_attn_info i;
   const int64_t* ks = k_start ? k_start->data() : nullptr;
   check_status(dh_attn_plan(q_len.data(), k_len.data(), ks, (int64_t)q_len.size(), (int)heads, (int)kv_heads, (int)head_dim, causal_block, nullptr, 0, &i),
-               "attention_plan (lengths and starts must not be negative, rows at most 2^30)");
+               "attention_plan (lengths and starts must not be negative, rows at most 2^30, work items a launch's)");
   torch::Tensor plan = torch::empty({i.ints}, torch::kInt32), info = torch::empty({(int64_t)(sizeof i / 8)}, torch::kInt64);
   check_status(dh_attn_plan(q_len.data(), k_len.data(), ks, (int64_t)q_len.size(), (int)heads, (int)kv_heads, (int)head_dim, causal_block,
                             plan.data_ptr<int32_t>(), i.ints, &i), "attention_plan");

@@ -369,7 +369,7 @@ template <typename Io, int V, bool ADJ, bool NORM> int launch(RopeParams& p, boo
   p.chunk = (total + parts - 1) / parts;
   const int gy = (total + p.chunk - 1) / p.chunk;
   if (!bwd) {
-    if (groups > 0x7fffffffl) return DH_ERR_ARG;
+    if (groups > 0xffffffffl / 256) return DH_ERR_ARG;                       // threads of one launch
     hipLaunchKernelGGL((rope_fwd_kernel<Io, V, ADJ, NORM>), dim3((unsigned)groups, gy), dim3(256), 0, st, p);
   } else {
     const int gx = (int)std::min<long>(groups, std::max(1, BWD_BLOCKS / gy));

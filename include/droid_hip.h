@@ -489,7 +489,7 @@ int dh_reproject_ex(const float* poses, const float* disps, const float* intrins
  * Outputs overlap neither inputs nor each other.
  *
  * dh_attn_plan runs on the HOST: it lays out the work items of one set of lengths.  plan_host NULL: only fills *info (info->ints = ints
- * wanted); else writes plan_host[0 .. info->ints).  The caller copies it to the device and passes it, with *info, to every call on these
+ * wanted); else writes plan_host[0 .. info->ints).  Up to 2^30 rows, and 2^32 threads (256 a work item and key head): DH_ERR_ARG beyond.  The caller copies it to the device and passes it, with *info, to every call on these
  * lengths.  Rows split over their keys (few rows, long key ranges) meet in the workspace.
  * o_low [q_rows, heads, head_dim] dense, or NULL: what the rounding of o to 16 bits left behind; the backward's row sums are formed from both.
  * dh_attn_bwd takes o, o_low and lse of the forward call with the same scale; sequences must not share keys (DH_ERR_ARG).  It is deterministic:
@@ -529,7 +529,8 @@ int dh_attn_bwd(const void* grad, int64_t g_st, int64_t g_sh, const void* q, int
  * sections[0] pairs turn by positions[:,0] * inv_freq[pair], the next sections[1] by positions[:,1], ...: (a, b) -> (a cos - b sin,
  * a sin + b cos); with P = sum of sections a pair is (i, P + i), or (2i, 2i + 1) where `interleaved`; channels from 2 P on do not turn.
  * An angle is off by 2^-51 of itself (64-bit product, reduced there), its sine and cosine by half a step of 32 bits (DH_F32) or 2.2e-7 (16-bit types).
- * head_dim even, up to 256 (above 128 the halves must be even: DH_ERR_UNSUPPORTED).
+ * head_dim even, up to 256 (above 128 the halves must be even: DH_ERR_UNSUPPORTED); up to 4096 heads and 4096 kv_heads.  Forward: as
+ * many tokens as 2^32 threads hold, 256 for 4 tokens (256 channels held singly) to 256 tokens: DH_ERR_ARG beyond.
  * Backward: x is only read where `normalize`; dq_weight / dk_weight [head_dim] of w_dtype or NULL; no atomics. */
 int dh_qk_norm_rope_fwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh,
                         void* q_out, int64_t qo_st, int64_t qo_sh, void* k_out, int64_t ko_st, int64_t ko_sh,

@@ -1,4 +1,5 @@
 """Token operators without a GPU: what a call refuses before it writes anything."""
+import ctypes
 import os
 import random
 import sys
@@ -77,3 +78,22 @@ def test_gradients_that_nobody_forms_are_refused():
                 at.qk_norm_rope(q, x, *a, [16])
         with torch.no_grad(), pytest.raises(RuntimeError, match="device tensor"):
             at.qk_norm_rope(x, x, *a, [16])
+
+
+def test_launches_of_too_many_threads_are_refused():
+    """before anything is launched (there is no GPU here: a launch would come back as another code)"""
+    lib = ctypes.CDLL(os.path.join(os.path.dirname(db.__file__), "libdroid_hip.so"))
+    i64, ptr, f32 = ctypes.c_int64, ctypes.c_void_p, ctypes.c_float
+    info = (i64 * 19)()
+
+    def plan(rows, kv):
+        return lib.dh_attn_plan((i64 * 1)(rows), (i64 * 1)(64), None, i64(1), kv, kv, 32, i64(0), None, i64(0), info)
+
+    assert plan(128 * 500000, 32) == 0                                       # 1.6 10^7 workgroups of 256
+    assert plan(128 * 600000, 32) == 1
+    sec, t = (ctypes.c_int * 1)(1), (ptr(256), i64(512), i64(256))
+
+    def rope(tokens, dim):
+        return lib.dh_qk_norm_rope_fwd(*t, *t, *t, *t, ptr(256), 0, ptr(256), sec, 1, ptr(0), ptr(0), 1, 0, i64(tokens), 1, 0, dim, 0, f32(1e-6), 1, ptr(0))
+
+    assert rope(2 ** 29 + 1, 256) == 1 and rope(2 ** 32 + 1, 2) == 1
