@@ -196,7 +196,8 @@ def audit_spills(force=False, verbose=False):
 
 
 def audit_m0(force=False, verbose=False):
-    """attention.hip sets m0 for its LDS-DMA in inline asm and does not restore it: require that nothing else in the generated ISA names m0."""
+    """attention.hip sets m0 for its LDS-DMA in inline asm and does not restore it: require that nothing else in the generated ISA names m0.  The compiler
+    does not look into the asm either: require that no vector instruction wrote the buffer's registers within the five wait states before the load."""
     import re
     src = os.path.join(CSRC, "attention.hip")
     stamp = os.path.join(OBJ, "attention.m0_audit_ok")
@@ -207,8 +208,20 @@ def audit_m0(force=False, verbose=False):
     lines = open(asm).read().splitlines()
     named = [i for i, l in enumerate(lines) if re.search(r"\bm0\b", l.split(";")[0])]
     bad = [lines[i] for i in named if not (lines[i].split()[:2] == ["s_mov_b32", "m0,"] and lines[i + 2].split()[0] == "buffer_load_dwordx4" and lines[i + 2].endswith("lds"))]
+    for i in (i + 2 for i in named if lines[i].split()[0] == "s_mov_b32" and not bad):
+        lo, hi = map(int, re.search(r"s\[(\d+):(\d+)\]", lines[i]).groups())
+        states, j = 0, i - 1
+        while states < 5 and j > 0:
+            t, j = lines[j].split(";")[0].strip(), j - 1
+            if re.match(r"s_nop ", t):
+                states += int(t.split()[1], 0) + 1
+            elif re.match(r"[a-z]\w* |s_barrier", t):
+                m = re.match(r"v_\w+ s(?:(\d+)|\[(\d+):(\d+)\])", t)
+                if m and int(m.group(1) or m.group(2)) <= hi and int(m.group(1) or m.group(3)) >= lo:
+                    bad.append("%s | %s" % (t, lines[i].strip()))
+                states += 1
     if bad or not named:
-        raise RuntimeError("m0 outside the LDS-DMA of attention.hip:\n" + "\n".join(bad[:10] or ["no LDS-DMA found"]))
+        raise RuntimeError("m0 outside the LDS-DMA of attention.hip, or a buffer written too shortly before it:\n" + "\n".join(bad[:10] or ["no LDS-DMA found"]))
     open(stamp, "w").write("%d LDS-DMA instructions\n" % len(named))
 
 
