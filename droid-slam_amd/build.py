@@ -250,12 +250,14 @@ def build_ext(force=False, verbose=False):
 
 
 def build_all(force=False, verbose=False):
-    build_lib(force, verbose)
-    if not SANITIZE:                      # (the ISA audits judge the release flags)
-        audit_asm_loads(force, verbose)
-        audit_spills(force, verbose)
-        audit_m0(force, verbose)
-    build_ext(force, verbose)
+    os.makedirs(OBJ, exist_ok=True)
+    audits = [] if SANITIZE else [audit_asm_loads, audit_spills, audit_m0]   # (the ISA audits judge the release flags; they compile listings of their own)
+    with ThreadPoolExecutor(max_workers=4) as ex:
+        running = [ex.submit(a, force, verbose) for a in audits]
+        build_lib(force, verbose)
+        build_ext(force, verbose)
+        for r in running:
+            r.result()
     return LIB, EXT
 
 
