@@ -20,7 +20,8 @@
 //
 // Precision.  Products of 16-bit operands accumulate in 32 bits; scores, statistics, p, dP, delta and all accumulators are 32-bit.
 // p and dS are rounded (to nearest) to the inputs' type as operands of the second product: their relative error is the same half step
-// that the rounding of the result has, and averages over the keys.  delta is a difference of large sums where the keys agree: it is formed
+// that the rounding of the result has, and averages over the keys; gradients are some 1.45 times as far from 64 bits as 32-bit sums rounded once
+// would be (results 1.0 to 1.1 times).  delta is a difference of large sums where the keys agree: it is formed
 // from o and what its rounding left behind (o_low; one more write and read of o's size), else dQ is off by 1.3 times as much.
 #include "common.h"
 #include <algorithm>
@@ -276,8 +277,8 @@ constexpr int CLEAR_BYTES = 1 << 15;             // a workgroup's share
 // One workgroup: NW x 32 rows (NW * 32 / group tokens) of one key head over the keys [begin, end) of its sequence.  Running maximum and sum
 // per row; the accumulator is only rescaled when a maximum grew by more than 2^8 (p <= 2^(TOP + 8) until then: exact in 32 bits, and a 16-bit p
 // keeps its relative precision, in fp16 down to 2^-21 of the largest).  slot >= 0: the row range is split over the keys, unnormalised sums go to the workspace for attn_join.
-// Bound by the matrix cores at the power limit (128 channels: 1.11 PFLOP/s on 19200 tokens, the library's large product 1.25), by the vector
-// units at 64 channels (0.72 on packed clips).
+// Bound by the matrix cores at the power limit (128 channels: 1.04 .. 1.11 PFLOP/s by card on 19200 tokens, the library's large product 1.25), by the vector
+// units at 64 channels (0.72 on packed clips, whose longest walks of 69 tiles also outlast a mean of 27: see dh_attn_plan).
 // How the keys come in: 64 keys a tile, one tile ahead; a lone wave (few rows, bound by memory: 82 us for 32 queries over 358 MB of keys, 4.4 TB/s)
 // takes 32 and keeps two tiles on their way in 48 KB, three waves a CU (90 us; with the same plan, two or four stages and as many waves as fit: 99, 95).
 template <int NW> struct Walk { static constexpr int BLOCKS = NW == 1 ? 1 : 2, STAGES = NW == 1 ? 3 : 2; };
@@ -928,7 +929,8 @@ __global__ __launch_bounds__(Dkv<DP>::WAVES * 64, DP == 128 ? 2 : 3) void attn_d
 #pragma unroll
       for (int i = 0; i < 16; ++i) dk[mb][i] *= a;
   }
-  if constexpr (Dkv<DP>::RW == 2) {                                          // the two halves of the rows meet in LDS, where the tiles were
+  {                                                                          // the two halves of the rows meet in LDS, where the tiles were
+    static_assert(Dkv<DP>::RW == 2, "two waves to a key");
     float* sum = reinterpret_cast<float*>(dyn) + wave * (DP * 64) + lane;
     __syncthreads();
     if (rw) {
@@ -1099,15 +1101,17 @@ extern "C" int dh_attn_plan(const int64_t* q_len, const int64_t* k_len, const in
     most = std::max<long>(most, q_len[i]);
     if (q_rows > MAX_ROWS || k_rows > MAX_ROWS || k_at > (1l << 40)) return DH_ERR_ARG;
   }
-  // rows a workgroup: one wave where a tile of 32 holds every row of the longest sequence, else 128 (32 single queries of 16/2 heads: 82 us against
+  // rows a workgroup, one choice for all sequences: one wave where a tile of 32 holds every row of the longest, else 128 (32 single queries of 16/2 heads: 82 us against
   // 109 with 128 rows; 768 queries of 8 heads over 23040 keys: 90 us against 59 with 128)
   const int waves = most * group <= 32 ? 1 : 4;
   const int tpt = waves * 32 / group, tpt_q = 128 / group;
   // Long walks over the keys become several work items (pieces of whole key tiles, joined afterwards) where they would outlast the rest:
   // the aim is an equal share of all key tiles for each of the workgroups that the chip holds at once.  A walk is only split if that saves
   // 24 tiles (some 20 us) of a workgroup's walk: a split row's sums go through memory once more, and the join is a launch of its own (packed clips,
-  // 64 channels: 87 us with 8, 85 with 24).  Lone waves are split for any saving: long walks meet short ones there, and a join is needed anyway (32
-  // queries over 1 .. 32400 keys: 82 us; 87 if it had to save 4 tiles, 130 if 24).
+  // 64 channels: 87 us with 8, 85 with 24).  The limit looks at each walk alone and is the same for every head_dim: on training clips (64 channels) walks of 36
+  // tiles stay whole beside a mean of 15, with all 648 workgroups on the chip at once, so that it empties while the longest end.
+  // Lone waves are split for any saving: long walks meet short ones there, and a join is needed anyway (32 queries over 1 .. 32400 keys: 82 us; 87 if it had to
+  // save 4 tiles, 130 if 24).
   const int dp = pad_dim(head_dim);
   struct Share {
     long piece, save;
