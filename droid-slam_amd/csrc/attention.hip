@@ -101,6 +101,7 @@ struct Params {
   long n_slots;
   int blocks, clear_q, clear_k;                  // workgroups of work items; from there on: rows [clear_q, q_rows) / [clear_k, k_rows) are cleared
   int kv_heads, group, heads, dim, block, q_rows, k_rows;
+  int plan_q_rows, plan_k_rows;                  // the rows that the plan's sequences have: what the workspaces are laid out for
   float c;                                       // scale * log2(e)
   float scale;
 };
@@ -225,9 +226,9 @@ __host__ __device__ __forceinline__ int keys_seen(int i, int q_len, int k_len, i
 // is one): there is no softmax of that
 __device__ __forceinline__ float row_factor(float l, int seen) { return seen <= 0 ? 0.f : l == 0.f ? NAN : 1.f / l; }
 
-__device__ __forceinline__ bool item_ok(const Item& it, const Params& p) {   // (holds for a plan of dh_attn_plan with these tensors)
+__device__ __forceinline__ bool item_ok(const Item& it, const Params& p) {   // (holds for every item of a plan with the info it came with)
   return it.q_start >= 0 && it.q_len >= 0 && it.k_start >= 0 && it.k_len >= 0 && it.first >= 0 && it.begin >= 0 &&
-         (long)it.q_start + it.q_len <= p.q_rows && (long)it.k_start + it.k_len <= p.k_rows;
+         (long)it.q_start + it.q_len <= p.plan_q_rows && (long)it.k_start + it.k_len <= p.plan_k_rows;
 }
 
 // acc += v^T p over 16 keys of which a row sees those below `lim` (lane's keys: from `key` on 4, and 4 more from key + 8 on).  p is 0 where a
@@ -1249,7 +1250,7 @@ extern "C" int dh_attn_fwd(const void* q, int64_t q_st, int64_t q_sh, const void
   if (info->n_slots && (!workspace || ((unsigned long)workspace & 15) || workspace_bytes < dh_attn_fwd_workspace_bytes(info))) return DH_ERR_WORKSPACE;
   p.low = (char*)o_low; p.lse = lse; p.part = (float*)workspace; p.n_slots = info->n_slots;
   p.kv_heads = (int)info->kv_heads; p.heads = (int)info->heads; p.group = p.heads / p.kv_heads; p.dim = dim; p.block = (int)info->causal_block;
-  p.q_rows = (int)q_rows; p.k_rows = (int)k_rows; p.clear_q = clear_rest ? (int)info->q_rows : p.q_rows; p.clear_k = clear_rest ? (int)info->k_rows : p.k_rows; p.scale = scale; p.c = scale * LOG2E;
+  p.q_rows = (int)q_rows; p.k_rows = (int)k_rows; p.plan_q_rows = (int)info->q_rows; p.plan_k_rows = (int)info->k_rows; p.clear_q = clear_rest ? (int)info->q_rows : p.q_rows; p.clear_k = clear_rest ? (int)info->k_rows : p.k_rows; p.scale = scale; p.c = scale * LOG2E;
   const Item* items = reinterpret_cast<const Item*>(plan);
   hipStream_t st = (hipStream_t)stream;
   const int dp = pad_dim(dim);
@@ -1291,7 +1292,7 @@ extern "C" int dh_attn_bwd(const void* grad, int64_t g_st, int64_t g_sh, const v
                       !view_ok(p.dv, k_rows, info->kv_heads, dim))) return DH_ERR_ARG;
   p.low = (char*)const_cast<void*>(o_low); p.lse = const_cast<float*>(lse); p.delta = (float*)workspace; p.row_values = info->q_rows * info->heads; p.part = (float*)workspace + row_floats(info);
   p.kv_heads = (int)info->kv_heads; p.heads = (int)info->heads; p.group = p.heads / p.kv_heads; p.dim = dim; p.block = (int)info->causal_block;
-  p.q_rows = (int)q_rows; p.k_rows = (int)k_rows; p.clear_q = clear_rest ? (int)info->q_rows : p.q_rows; p.clear_k = clear_rest ? (int)info->k_rows : p.k_rows; p.scale = scale; p.c = scale * LOG2E;
+  p.q_rows = (int)q_rows; p.k_rows = (int)k_rows; p.plan_q_rows = (int)info->q_rows; p.plan_k_rows = (int)info->k_rows; p.clear_q = clear_rest ? (int)info->q_rows : p.q_rows; p.clear_k = clear_rest ? (int)info->k_rows : p.k_rows; p.scale = scale; p.c = scale * LOG2E;
   const Item* items = reinterpret_cast<const Item*>(plan);
   hipStream_t st = (hipStream_t)stream;
   const int dp = pad_dim(dim);

@@ -485,6 +485,7 @@ int dh_reproject_ex(const float* poses, const float* disps, const float* intrins
  * Rows behind the last sequence (of o, lse, dq) and behind the last key (of dk, dv) are left as they were, or cleared where clear_rest
  * (o, gradients 0, lse -inf).  Rows of dk, dv between the sequences' keys (k_start with gaps) are left as they were.
  * Scores (scale q.k) up to 10^8 in size, gradients too.  Values are expected to be finite where a gradient is wanted (rows that see nothing may hold anything).  A non-finite value (q, k or v) reaches the rows that see it and no others.
+ * Sums of v have to fit 32 bits with a factor of 2^8 (bf16 values up to 10^30 do).
  *
  * Outputs overlap neither inputs nor each other.
  *
@@ -531,6 +532,7 @@ int dh_attn_bwd(const void* grad, int64_t g_st, int64_t g_sh, const void* q, int
  * An angle is off by 2^-51 of itself (64-bit product, reduced there), its sine and cosine by half a step of 32 bits (DH_F32) or 2.2e-7 (16-bit types).
  * head_dim even, up to 256 (above 128 the halves must be even: DH_ERR_UNSUPPORTED); up to 4096 heads and 4096 kv_heads.  Forward: as
  * many tokens as 2^32 threads hold, 256 for 4 tokens (256 channels held singly) to 256 tokens: DH_ERR_ARG beyond.
+ * The sum of x^2 has to fit 32 bits (|x| up to 10^18; from 10^-18 on where eps = 0).
  * Backward: x is only read where `normalize`; dq_weight / dk_weight [head_dim] of w_dtype or NULL; no atomics. */
 int dh_qk_norm_rope_fwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh,
                         void* q_out, int64_t qo_st, int64_t qo_sh, void* k_out, int64_t ko_st, int64_t ko_sh,

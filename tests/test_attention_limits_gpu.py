@@ -1,4 +1,5 @@
 """Token operators on the GPU at the ends of their range: results against the definition, within bounds that follow from the roundings."""
+import ctypes
 import os
 import sys
 
@@ -228,3 +229,29 @@ def test_out_is_seen_by_autograd():
     with torch.inference_mode():
         out = torch.empty_like(q)
         assert torch.equal(at.packed_attention(q, k, v, plan, out=out), at.packed_attention(q, k, v, plan))
+
+
+def test_a_plan_with_another_plans_info_stays_inside_the_workspace():
+    """as many items, other lengths: what reaches behind the rows of the info is left out, forward and backward, whatever rows the tensors have"""
+    lib = ctypes.CDLL(os.path.join(os.path.dirname(at.droid_backends.__file__), "libdroid_hip.so"))
+    i64, ptr, f32 = ctypes.c_int64, ctypes.c_void_p, ctypes.c_float
+    lib.dh_attn_bwd_workspace_bytes.restype = ctypes.c_size_t
+    h, kv, d, rows = 4, 2, 64, 40
+    q, k, v, g = inputs([rows], None, h, kv, d, F16, 5)
+    info, other = (i64 * 19)(), (i64 * 19)()
+    items = (ctypes.c_int32 * 24)()
+    one = lambda n: (i64 * 1)(n)  # noqa: E731
+    assert lib.dh_attn_plan(one(8), one(8), None, i64(1), h, kv, d, i64(0), None, i64(0), info) == 0
+    assert lib.dh_attn_plan(one(31), one(31), None, i64(1), h, kv, d, i64(0), items, i64(24), other) == 0 and info[0] == other[0] == 24
+    items = torch.frombuffer(items, dtype=torch.int32).clone().cuda()
+    n = lib.dh_attn_bwd_workspace_bytes(info)
+    ws = torch.full((n // 4 + 4096,), 7.0, device="cuda")
+    o, dq, lse = torch.full_like(q, 7.0), torch.full_like(q, 7.0), torch.full((rows, h), 7.0, device="cuda")
+    dk, dv = torch.full_like(k, 7.0), torch.full_like(k, 7.0)
+    t = lambda x: (ptr(x.data_ptr()), i64(x.stride(0)), i64(x.stride(1)))  # noqa: E731
+    p = lambda x: ptr(x.data_ptr())  # noqa: E731
+    tail = (p(items), info, 0, i64(rows), i64(rows), f32(0.125), 0, p(ws), ctypes.c_size_t(n), ptr(torch.cuda.current_stream().cuda_stream))
+    assert lib.dh_attn_fwd(*t(q), *t(k), *t(v), *t(o), ptr(0), p(lse), *tail) == 0
+    assert lib.dh_attn_bwd(*t(g), *t(q), *t(k), *t(v), *t(o), ptr(0), p(lse), *t(dq), *t(dk), *t(dv), *tail) == 0
+    torch.cuda.synchronize()
+    assert all(bool((x == 7).all()) for x in (o, lse, dq, dk, dv, ws[n // 4:]))
